@@ -14,29 +14,22 @@
 // Every wait on an mbarrier is bounded by a wall-clock deadline; a wait that gives up raises an
 // abort flag, records a code in the context's status word, drains the CTA's own copies and MMAs,
 // frees TMEM and returns, so a faulty launch cannot hang the GPU.
-#include <cuda.h>
-
-#include <mutex>
-
 #include "cf_common.cuh"
 #include "cf_gemm.cuh"
+#include "cf_tc.cuh"
 
 namespace cf {
 namespace {
 
+using namespace tc;
+
 constexpr int BM = 128;                 // rows of A / C per CTA (TMEM lanes)
 constexpr int BN = 256;                 // output columns per tile
-constexpr int BK = 128;                 // bytes == FP8 elements per k-block (one 128B swizzle row)
-constexpr int UMMA_K = 32;              // FP8 elements per tcgen05.mma
 constexpr int NUM_THREADS = 320;        // warp 0 producer, warp 1 MMA issuer, warps 2..9 epilogue
 constexpr int EPI_WARPS = 8;            // two per TMEM lane quarter: each handles 128 of the tile's 256 columns
 constexpr int TMEM_COLS = 512;          // two 128x256 fp32 accumulators per CTA
-constexpr unsigned long long WAIT_NS = 1500ull * 1000ull * 1000ull;   // per-wait deadline
-constexpr unsigned long long DRAIN_NS = 20ull * 1000ull * 1000ull;
 
-// Output staging for the TMA-store epilogue: per epilogue warp one 32-row x 128-byte (64 bf16) box.
-constexpr int C_BOX_COLS = 64;
-constexpr int C_BOX_BYTES = 32 * C_BOX_COLS * 2;           // 4 KiB
+// Output staging for the TMA-store epilogue: one box per epilogue warp.
 constexpr int C_STAGING = EPI_WARPS * C_BOX_BYTES;         // 32 KiB
 
 // Shape of the shared-memory ring. Single CTA: the CTA loads all 256 rows of the B tile. CTA pair
@@ -52,167 +45,6 @@ struct Cfg {
     static constexpr int RING = STAGES * (A_STAGE + B_STAGE);
     static constexpr int SMEM_BYTES = RING + C_STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/;
 };
-
-// ------------------------------------------------------------------ PTX wrappers
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ unsigned long long gtime_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait. Returns false when the deadline passed or another role of this CTA aborted.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* s_abort,
-                                          unsigned long long limit_ns = WAIT_NS) {
-    for (int i = 0; i < 64; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = gtime_ns();
-    while (true) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*s_abort) return false;
-        if (gtime_ns() - t0 > limit_ns) return false;
-        __nanosleep(64);
-    }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-// The output is written once and not read again by this kernel: evict-first keeps it from pushing the operand
-// slabs (which every tile re-reads) out of L2.
-__device__ __forceinline__ uint64_t l2_policy_evict_first() {
-    uint64_t pol;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
-    return pol;
-}
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y, uint64_t policy) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;"
-                 ::"l"(map), "r"(src), "r"(x), "r"(y), "l"(policy) : "memory");
-}
-// fp32 accumulate (beta = 1) as a TMA reduction: the staged tile is added to global memory in L2, one addition per
-// element like a read-modify-write epilogue, but with whole 128-byte lines.
-__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
-    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
-                 ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read_0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ void tcgen05_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// Pair form: the arrive is delivered to the barrier at the same offset in both CTAs of the pair.
-__device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
-    const uint16_t mask = 3;
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"(mask) : "memory");
-}
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// shared::cluster address of `local_addr` in CTA `rank` of this cluster
-__device__ __forceinline__ uint32_t mapa(uint32_t local_addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local_addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Pair form of the TMA load: the data lands in this CTA's shared memory, the byte count is credited to a
-// barrier that may live in the other CTA of the pair (no multicast: every CTA fetches its own box).
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar_cluster), "r"(x), "r"(y)
-        : "memory");
-}
-__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// K-major operand tile in shared memory, rows of 128 bytes, 128B swizzle (what the TMA box writes):
-// start address >> 4 in bits [0,14), leading byte offset (unused for swizzled K-major) = 1 in [16,30),
-// stride byte offset = 8 rows * 128 B = 1024 B >> 4 in [32,46), descriptor version 1 in [46,48),
-// layout type 2 (SWIZZLE_128B) in [61,64).
-__device__ __forceinline__ uint64_t make_smem_desc(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((saddr & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>(1) << 16;
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(2) << 61;
-    return d;
-}
-
-// kind::f8f6f4 instruction descriptor: D fp32 (bits 4-5 = 1), A format bits 7-9, B format bits 10-12
-// (0 = E4M3, 1 = E5M2), both operands K-major (bits 15,16 = 0), N>>3 in bits 17-22, M>>4 in bits 24-28.
-// An MN-major operand lies in shared memory with the rows of the tile running along K and 128 contiguous bytes along
-// M / N: bit 15 for A, bit 16 for B.
-__device__ __forceinline__ uint32_t make_idesc(int a_e5m2, int b_e5m2, int mma_m, int a_mn_major, int b_mn_major) {
-    return (1u << 4) | (static_cast<uint32_t>(a_e5m2) << 7) | (static_cast<uint32_t>(b_e5m2) << 10) |
-           (a_mn_major ? (1u << 15) : 0u) | (b_mn_major ? (1u << 16) : 0u) |
-           (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(mma_m >> 4) << 24);
-}
-
 
 struct TileCoord {
     int row0;        // first global row of A / C for this tile
@@ -295,11 +127,6 @@ __device__ __forceinline__ float swiglu_sigmoid(float x) {
     // one IEEE division with the matching numerator gives the same bits without a divergent branch.
     const float e = expf(-fabsf(x));
     return __fdiv_rn(x >= 0.0f ? 1.0f : e, 1.0f + e);
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
 }
 // max(a, |b|) on two packed bf16 values (a holds non-negative values); a NaN in b leaves a unchanged, like fmaxf.
 __device__ __forceinline__ uint32_t bf16x2_absmax(uint32_t a, uint32_t b) {
@@ -458,7 +285,7 @@ k_gemm_fp8_nt(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         if (lane == 0 && leader) {
             const bool mn = WIDE && p.mn_major;
             const bool bmn = WIDE && (p.mn_major || p.b_mn_major);
-            const uint32_t idesc = make_idesc(p.a_e5m2, p.b_e5m2, TM, mn, bmn);
+            const uint32_t idesc = make_idesc(p.a_e5m2, p.b_e5m2, TM, BN, mn, bmn);
             int it = 0, local_tile = 0;
             bool ok = true;
             for (int tile = unit; ok && tile < total_tiles; tile += n_units, ++local_tile) {
@@ -946,38 +773,6 @@ __global__ void __launch_bounds__(256) k_gemm_fp8_nt_simt(const uint8_t* __restr
 }
 
 // ------------------------------------------------------------------ host side
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
-
-// 2-D byte tensor [rows, K] with row pitch `pitch`, box {BK, box_rows}, 128B swizzle, zero fill out of bounds.
-int make_map(CUtensorMap* map, const void* ptr, long long rows, long long K, long long pitch, int box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) { set_error("cuTensorMapEncodeTiled entry point not available"); return CF_ERR_CUDA; }
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    const cuuint32_t box[2] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box_rows)};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r)); return CF_ERR_CUDA; }
-    return CF_OK;
-}
-
 // Number of CTA pairs the device can keep resident at once (cached per device); 0 = pairs unusable.
 int max_resident_pairs() {
     static int cached[64];
@@ -1003,36 +798,6 @@ int max_resident_pairs() {
         cached[dev & 63] = n;
     });
     return cached[dev & 63];
-}
-
-// bf16 output tensor [rows, N] with row pitch ldc elements, box {64 columns, 32 rows}, 128B swizzle.
-int make_map_c(CUtensorMap* map, const void* ptr, long long rows, long long N, long long ldc) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) { set_error("cuTensorMapEncodeTiled entry point not available"); return CF_ERR_CUDA; }
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc) * 2};
-    const cuuint32_t box[2] = {static_cast<cuuint32_t>(C_BOX_COLS), 32};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled (output) failed with CUresult %d", static_cast<int>(r)); return CF_ERR_CUDA; }
-    return CF_OK;
-}
-
-// fp32 accumulator tensor [rows, N] with row pitch ldc elements, box {32 columns, 32 rows}, 128B swizzle.
-int make_map_c_f32(CUtensorMap* map, const void* ptr, long long rows, long long N, long long ldc) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) { set_error("cuTensorMapEncodeTiled entry point not available"); return CF_ERR_CUDA; }
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc) * 4};
-    const cuuint32_t box[2] = {32, 32};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled (fp32 output) failed with CUresult %d", static_cast<int>(r)); return CF_ERR_CUDA; }
-    return CF_OK;
 }
 
 }  // namespace
