@@ -19,6 +19,7 @@ fp = C.c_void_p      # float* on the device
 ip = C.c_void_p      # int* on the device
 sz = C.c_size_t
 ci = C.c_int
+ll = C.c_longlong
 cf = C.c_float
 
 
@@ -115,6 +116,17 @@ SIGNATURES = {
     "cf_fp8_quantize_rowwise_e4m3": (ci, [vp, ci, vp, ci, fp, fp, ci, ci, vp]),
     "cf_swiglu_quantize_rowwise_e4m3": (ci, [vp, vp, ci, vp, ci, fp, fp, ci, ci, vp]),
     "cf_swiglu_quantize_e4m3_record": (ci, [vp, vp, ci, vp, ci, fp, fp, ci, ci, vp]),
+    "cf_fp8_quantize_block128": (ci, [vp, ci, ci, ci, ci, vp, ci, fp, ll, ll, vp, ci, fp, ll, ll, vp]),
+    "cf_swiglu_quantize_block128": (ci, [vp, vp, ci, ci, ci, vp, ci, fp, ll, ll, vp, ci, fp, ll, ll, vp]),
+    "cf_swiglu_backward_quantize_block128": (ci, [vp, vp, ci, vp, ci, ci, ci, ci, vp, ci, fp, ll, ll, vp, ci, fp, ll, ll, vp]),
+    "cf_fp8_quantize_block128x128": (ci, [vp, ci, ll, ci, ci, ci, vp, ci, ll, fp, ll, ll, vp]),
+    "cf_add_rmsnorm_quantize_block128": (ci, [vp, vp, vp, vp, vp, fp, vp, ci, fp, ll, ll, ci, ci, cf, vp]),
+    "cf_add_rmsnorm_backward_scratch_floats": (sz, [ci, ci]),
+    "cf_add_rmsnorm_backward": (ci, [vp, vp, vp, fp, vp, vp, fp, ci, fp, sz, ci, ci, vp]),
+    "cf_gemm_fp8_block128_nt": (ci, [vp, ci, ci, ci, vp, ci, ci, fp, ll, ll, vp, ci, fp, ll, ll, ci, vp, ci, ci, ci, vp]),
+    "cf_gemm_fp8_block128_nt_grouped": (ci, [vp, ci, ci, ci, ci, ip, ip, vp, ci, ci, fp, ll, ll, vp, ci, fp, ll, ll, vp, ci, vp]),
+    "cf_gemm_fp8_block128_nn": (ci, [vp, ci, ci, ci, vp, ci, ci, fp, ll, ll, vp, ci, fp, ll, vp, ci, ci, ci, vp]),
+    "cf_gemm_fp8_block128_dw": (ci, [vp, ci, ci, ci, vp, ci, ci, fp, ll, ll, vp, ci, ci, fp, ll, ll, vp, ci, ci, ci, vp]),
     "cf_moe_topk_route_f32": (ci, [fp, ci, ci, ci, vp, fp, fp, ci]),
     "cf_moe_build_expert_row_lists": (ci, [fp, ip, ip, ci, ci, vp]),
     "cf_moe_expert_offsets_from_counts": (ci, [ip, ip, ci, vp]),

@@ -1,0 +1,373 @@
+// Block-scaled FP8 quantiser: one fp32 scale for every group of 128 values.
+//
+//   a = max(max|v| over the group, 1e-12),  descale = a / FMAX,  code = fp8(v * (FMAX / a))      FMAX = 448 or 57344
+//
+// Groups run along a row (1x128: operands whose contraction runs along the row), down a column (128x1: operands of the
+// weight gradient, contracted over tokens) or are 128x128 blocks (weights). v is a bf16 matrix, silu(gate) * up, or the
+// gradient of silu(gate) * up. Products and amax are taken in fp32 and rounded ONCE, to the code: the descale is held in
+// 32 bits, and no bf16 rounding lies between the activation and its code.
+// The reference scales per tensor only; the formulas generalise kernels/fp8.cu:34-49 to groups.
+//
+// All forms are streams: they are bound by the bytes of inputs and codes (2 B in + 1 B out per element and output of the
+// plain form), so every input element is read once whatever the number of outputs. A block owns a tile of 128 columns;
+// a half-warp reads 128 columns of one row (256 contiguous bytes) and holds that row's group, so the row amax is four
+// shuffles; the column amax meets in shared memory across the rows of the tile; the values stay in registers in between.
+#include "cf_common.cuh"
+#include "cf_internal.cuh"
+
+namespace cf {
+namespace {
+
+constexpr int G = 128;                       // values per scale
+constexpr float kFloorAmax = 1e-12f;
+
+enum Src { SRC_PLAIN = 0, SRC_SWIGLU = 1, SRC_SWIGLU_GRAD = 2 };
+
+struct QuantParams {
+    const uint16_t* x;        // plain source, or gate
+    const uint16_t* up;
+    const uint16_t* dh;
+    long long ld_x;           // row pitch of x / gate / up in elements
+    long long ld_dh;
+    int rows, cols;           // of the source
+    uint8_t* row8;
+    long long ld_row8;
+    float* row_d;
+    long long rd_row, rd_blk; // strides of the row descales
+    uint8_t* col8;
+    long long ld_col8;
+    float* col_d;
+    long long cd_blk, cd_col; // strides of the column descales
+    int col_blocks;
+    int vec_in, vec_row8, vec_col8;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+    f[4] = __uint_as_float(v.z << 16); f[5] = __uint_as_float(v.z & 0xffff0000u);
+    f[6] = __uint_as_float(v.w << 16); f[7] = __uint_as_float(v.w & 0xffff0000u);
+}
+// Eight bf16 values of a row as one 16-byte load, or element by element where the row's base or its end forbid that.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int n, bool vec) {
+    if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= static_cast<uint32_t>(__ldg(p + e)) << (16 * (e & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(uint8_t* p, const uint2& q, int n, bool vec) {
+    if (vec && n >= 8) { *reinterpret_cast<uint2*>(p) = q; return; }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) p[e] = static_cast<uint8_t>((e < 4 ? q.x >> (8 * e) : q.y >> (8 * (e - 4))) & 0xffu);
+}
+template <bool E5M2>
+__device__ __forceinline__ uint2 code8(const float (&f)[8], float s) {
+    return make_uint2(cvt_fp8x4<E5M2>(f[0] * s, f[1] * s, f[2] * s, f[3] * s), cvt_fp8x4<E5M2>(f[4] * s, f[5] * s, f[6] * s, f[7] * s));
+}
+template <bool E5M2>
+__device__ __forceinline__ uint2 code8c(const float (&f)[8], const float (&s)[8]) {
+    return make_uint2(cvt_fp8x4<E5M2>(f[0] * s[0], f[1] * s[1], f[2] * s[2], f[3] * s[3]),
+                      cvt_fp8x4<E5M2>(f[4] * s[4], f[5] * s[5], f[6] * s[6], f[7] * s[7]));
+}
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+    return v;
+}
+__device__ __forceinline__ float sigmoid_f(float x) {
+    const float e = expf(-fabsf(x));        // no overflow on either side of zero
+    return __fdiv_rn(x >= 0.0f ? 1.0f : e, 1.0f + e);
+}
+
+// One half of the outputs of a tile: `f` holds RPT rows x 8 columns per thread, row i of the thread at r0 + rg + i * RG.
+// cb: column block of the output (the SwiGLU gradient's second half is shifted by the width of the first).
+template <int T, int RPT, bool ROW, bool COL, bool E5M2>
+__device__ __forceinline__ void emit_tile(const QuantParams& p, float (&f)[RPT][8], int r0, int c0, int shift, float* s_col) {
+    constexpr int RG = T / 16;
+    constexpr float FMAX = E5M2 ? 57344.0f : 448.0f;
+    const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
+    const int col = c0 + cg * 8;
+    const int n = min(8, p.cols - col);
+    if (ROW) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = r0 + rg + i * RG;
+            float a = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(f[i][e]));
+            a = fmaxf(half_warp_max(a), kFloorAmax);
+            if (r < p.rows && n > 0) {
+                store8(p.row8 + static_cast<long long>(r) * p.ld_row8 + shift + col, code8<E5M2>(f[i], __fdiv_rn(FMAX, a)), n, p.vec_row8);
+                if (cg == 0) p.row_d[r * p.rd_row + ((shift + c0) / G) * p.rd_blk] = __fdiv_rn(a, FMAX);
+            }
+        }
+    }
+    if (COL) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        float m[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m[e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) m[e] = fmaxf(m[e], fabsf(f[i][e]));
+            m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
+        }
+        if (lane < 16) {
+            float4* d = reinterpret_cast<float4*>(s_col + warp * G + cg * 8);
+            d[0] = make_float4(m[0], m[1], m[2], m[3]);
+            d[1] = make_float4(m[4], m[5], m[6], m[7]);
+        }
+        __syncthreads();
+        float* s_scale = s_col + (T / 32) * G;
+        if (threadIdx.x < G) {
+            float a = s_col[threadIdx.x];
+#pragma unroll
+            for (int w = 1; w < T / 32; ++w) a = fmaxf(a, s_col[w * G + threadIdx.x]);
+            a = fmaxf(a, kFloorAmax);
+            s_scale[threadIdx.x] = __fdiv_rn(FMAX, a);
+            if (c0 + static_cast<int>(threadIdx.x) < p.cols)
+                p.col_d[(r0 / G) * p.cd_blk + static_cast<long long>(shift + c0 + threadIdx.x) * p.cd_col] = __fdiv_rn(a, FMAX);
+        }
+        __syncthreads();
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = s_scale[cg * 8 + e];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = r0 + rg + i * RG;
+            if (r < p.rows && n > 0)
+                store8(p.col8 + static_cast<long long>(r) * p.ld_col8 + shift + col, code8c<E5M2>(f[i], s), n, p.vec_col8);
+        }
+        __syncthreads();            // the SwiGLU gradient comes back for its second half
+    }
+}
+
+// Tile of (T / 16) * RPT rows x 128 columns. With column groups the tile has 128 rows.
+template <int SRC, int T, int RPT, bool ROW, bool COL, bool E5M2>
+__global__ void __launch_bounds__(T) k_quant_block128(const QuantParams p) {
+    constexpr int RG = T / 16;
+    __shared__ __align__(16) float s_col[COL ? (T / 32 + 1) * G : 4];
+    const int cb = blockIdx.x % p.col_blocks, rb = blockIdx.x / p.col_blocks;
+    const int c0 = cb * G, r0 = rb * (RG * RPT);
+    const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
+    const int col = c0 + cg * 8;
+    const int n = min(8, p.cols - col);
+
+    uint4 a[RPT], b[SRC != SRC_PLAIN ? RPT : 1], d[SRC == SRC_SWIGLU_GRAD ? RPT : 1];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = r0 + rg + i * RG;
+        a[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (SRC != SRC_PLAIN) b[i] = a[i];
+        if (SRC == SRC_SWIGLU_GRAD) d[i] = a[i];
+        if (r < p.rows && n > 0) {
+            a[i] = load8(p.x + r * p.ld_x + col, n, p.vec_in);
+            if (SRC != SRC_PLAIN) b[i] = load8(p.up + r * p.ld_x + col, n, p.vec_in);
+            if (SRC == SRC_SWIGLU_GRAD) d[i] = load8(p.dh + r * p.ld_dh + col, n, p.vec_in);
+        }
+    }
+    float f[RPT][8];
+    if (SRC == SRC_PLAIN) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) unpack8(a[i], f[i]);
+        emit_tile<T, RPT, ROW, COL, E5M2>(p, f, r0, c0, 0, s_col);
+    } else if (SRC == SRC_SWIGLU) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            float u[8];
+            unpack8(a[i], f[i]);
+            unpack8(b[i], u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * sigmoid_f(f[i][e]) * u[e];
+        }
+        emit_tile<T, RPT, ROW, COL, E5M2>(p, f, r0, c0, 0, s_col);
+    } else {
+        // d gate = dh up sig(g) (1 + g (1 - sig(g))),  d up = dh g sig(g): the two halves of one [rows, 2 cols] gradient
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+                float g[8], w[8];
+                unpack8(a[i], g);
+                unpack8(d[i], f[i]);
+                if (half == 0) unpack8(b[i], w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float sg = sigmoid_f(g[e]);
+                    f[i][e] *= half == 0 ? w[e] * sg * (1.0f + g[e] * (1.0f - sg)) : g[e] * sg;
+                }
+            }
+            emit_tile<T, RPT, ROW, COL, E5M2>(p, f, r0, c0, half * p.cols, s_col);
+        }
+    }
+}
+
+// Weights: one scale per 128x128 block of every [rows, cols] matrix of a stack (blocks restart in each matrix).
+constexpr int kWT = 512;
+__global__ void __launch_bounds__(kWT) k_quant_block128x128(const uint16_t* __restrict__ w, long long ld_w, long long w_stride, int rows,
+                                                            int cols, int row_blocks, int col_blocks, uint8_t* __restrict__ out,
+                                                            long long ld_out, long long out_stride, float* __restrict__ descale,
+                                                            long long d_row, long long d_stride, int vec_in, int vec_out) {
+    constexpr int RG = kWT / 16, RPT = G / RG;
+    __shared__ float s_part[kWT / 32];
+    const int cb = blockIdx.x % col_blocks;
+    const int t = blockIdx.x / col_blocks;
+    const int rb = t % row_blocks, m = t / row_blocks;
+    const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
+    const int col = cb * G + cg * 8;
+    const int n = min(8, cols - col);
+    const uint16_t* src = w + m * w_stride;
+    uint4 v[RPT];
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = rb * G + rg + i * RG;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows && n > 0) v[i] = load8(src + r * ld_w + col, n, vec_in);
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        float f[8];
+        unpack8(v[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(f[e]));
+    }
+    a = warp_max(a);
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = s_part[0];
+#pragma unroll
+    for (int i = 1; i < kWT / 32; ++i) a = fmaxf(a, s_part[i]);
+    a = fmaxf(a, kFloorAmax);
+    const float s = __fdiv_rn(448.0f, a);
+    if (threadIdx.x == 0) descale[m * d_stride + rb * d_row + cb] = __fdiv_rn(a, 448.0f);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = rb * G + rg + i * RG;
+        if (r < rows && n > 0) {
+            float f[8];
+            unpack8(v[i], f);
+            store8(out + m * out_stride + r * ld_out + col, code8<false>(f, s), n, vec_out);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+
+template <int SRC, int T, int RPT, bool ROW, bool COL>
+int launch_fmt(const QuantParams& p, int e5m2, cudaStream_t st) {
+    const long long blocks = cdiv(p.rows, (T / 16) * RPT) * p.col_blocks;
+    if (blocks > 0x7fffffffll) { set_error("block-128 quantiser: matrix too large for one launch"); return CF_ERR_LIMIT; }
+    if (e5m2) k_quant_block128<SRC, T, RPT, ROW, COL, true><<<static_cast<unsigned>(blocks), T, 0, st>>>(p);
+    else k_quant_block128<SRC, T, RPT, ROW, COL, false><<<static_cast<unsigned>(blocks), T, 0, st>>>(p);
+    CF_LAUNCH_CHECK("quant_block128");
+    return CF_OK;
+}
+
+template <int SRC>
+int launch_quant(const char* fn, QuantParams p, int e5m2, int halves, cudaStream_t st) {
+    CF_REQUIRE(p.rows >= 0 && p.cols >= 0, "%s: negative shape", fn);
+    if (p.rows == 0 || p.cols == 0) return CF_OK;
+    if (p.rows > 0x7fff0000 || p.cols > 0x3fff0000) { set_error("%s: more than 2^31 rows or 2^30 columns", fn); return CF_ERR_LIMIT; }
+    const bool row = p.row8 != nullptr, col = p.col8 != nullptr;
+    CF_REQUIRE(row || col, "%s: no output", fn);
+    CF_REQUIRE(row == (p.row_d != nullptr) && col == (p.col_d != nullptr), "%s: codes and descales go together", fn);
+    CF_REQUIRE(p.x && (SRC == SRC_PLAIN || p.up) && (SRC != SRC_SWIGLU_GRAD || p.dh), "%s: null input", fn);
+    CF_REQUIRE(p.ld_x >= p.cols && (SRC != SRC_SWIGLU_GRAD || p.ld_dh >= p.cols), "%s: input pitch smaller than a row", fn);
+    CF_REQUIRE((!row || p.ld_row8 >= static_cast<long long>(halves) * p.cols) && (!col || p.ld_col8 >= static_cast<long long>(halves) * p.cols),
+               "%s: output pitch smaller than a row", fn);
+    CF_REQUIRE(halves == 1 || p.cols % G == 0, "%s: the two halves need cols to be a multiple of 128", fn);
+    CF_REQUIRE(aligned(p.x, 2) && aligned(p.up, 2) && aligned(p.dh, 2) && aligned(p.row_d, 4) && aligned(p.col_d, 4),
+               "%s: misaligned pointer", fn);
+    const int rc = require_sm100();
+    if (rc != CF_OK) return rc;
+    p.col_blocks = static_cast<int>(cdiv(p.cols, G));
+    p.vec_in = aligned(p.x, 16) && aligned(p.up, 16) && aligned(p.dh, 16) && p.ld_x % 8 == 0 && (SRC != SRC_SWIGLU_GRAD || p.ld_dh % 8 == 0);
+    p.vec_row8 = row && aligned(p.row8, 8) && p.ld_row8 % 8 == 0;
+    p.vec_col8 = col && aligned(p.col8, 8) && p.ld_col8 % 8 == 0;
+    if (col && row) return launch_fmt<SRC, 512, 4, true, true>(p, e5m2, st);
+    if (col) return launch_fmt<SRC, 512, 4, false, true>(p, e5m2, st);
+    return launch_fmt<SRC, 128, 2, true, false>(p, e5m2, st);
+}
+
+}  // namespace
+}  // namespace cf
+
+using namespace cf;
+
+extern "C" {
+
+int cf_fp8_quantize_block128(const void* d_x, int ld_x, int rows, int cols, int is_e5m2, void* d_row8_or_null, int ld_row8,
+                             float* d_row_descale, long long row_descale_ld_row, long long row_descale_ld_block, void* d_col8_or_null,
+                             int ld_col8, float* d_col_descale, long long col_descale_ld_block, long long col_descale_ld_col, void* stream) {
+    QuantParams p = {};
+    p.x = static_cast<const uint16_t*>(d_x); p.ld_x = ld_x; p.rows = rows; p.cols = cols;
+    p.row8 = static_cast<uint8_t*>(d_row8_or_null); p.ld_row8 = ld_row8;
+    p.row_d = d_row_descale; p.rd_row = row_descale_ld_row; p.rd_blk = row_descale_ld_block;
+    p.col8 = static_cast<uint8_t*>(d_col8_or_null); p.ld_col8 = ld_col8;
+    p.col_d = d_col_descale; p.cd_blk = col_descale_ld_block; p.cd_col = col_descale_ld_col;
+    return launch_quant<SRC_PLAIN>("cf_fp8_quantize_block128", p, is_e5m2, 1, as_stream(stream));
+}
+
+int cf_swiglu_quantize_block128(const void* d_gate, const void* d_up, int ld_in, int rows, int cols, void* d_row8_or_null, int ld_row8,
+                                float* d_row_descale, long long row_descale_ld_row, long long row_descale_ld_block,
+                                void* d_col8_or_null, int ld_col8, float* d_col_descale, long long col_descale_ld_block,
+                                long long col_descale_ld_col, void* stream) {
+    QuantParams p = {};
+    p.x = static_cast<const uint16_t*>(d_gate); p.up = static_cast<const uint16_t*>(d_up);
+    p.ld_x = ld_in; p.rows = rows; p.cols = cols;
+    p.row8 = static_cast<uint8_t*>(d_row8_or_null); p.ld_row8 = ld_row8;
+    p.row_d = d_row_descale; p.rd_row = row_descale_ld_row; p.rd_blk = row_descale_ld_block;
+    p.col8 = static_cast<uint8_t*>(d_col8_or_null); p.ld_col8 = ld_col8;
+    p.col_d = d_col_descale; p.cd_blk = col_descale_ld_block; p.cd_col = col_descale_ld_col;
+    return launch_quant<SRC_SWIGLU>("cf_swiglu_quantize_block128", p, 0, 1, as_stream(stream));
+}
+
+int cf_swiglu_backward_quantize_block128(const void* d_gate, const void* d_up, int ld_in, const void* d_dh, int ld_dh, int rows, int cols,
+                                         int is_e5m2, void* d_row8_or_null, int ld_row8, float* d_row_descale,
+                                         long long row_descale_ld_row, long long row_descale_ld_block, void* d_col8_or_null,
+                                         int ld_col8, float* d_col_descale, long long col_descale_ld_block, long long col_descale_ld_col,
+                                         void* stream) {
+    QuantParams p = {};
+    p.x = static_cast<const uint16_t*>(d_gate); p.up = static_cast<const uint16_t*>(d_up); p.dh = static_cast<const uint16_t*>(d_dh);
+    p.ld_x = ld_in; p.ld_dh = ld_dh; p.rows = rows; p.cols = cols;
+    p.row8 = static_cast<uint8_t*>(d_row8_or_null); p.ld_row8 = ld_row8;
+    p.row_d = d_row_descale; p.rd_row = row_descale_ld_row; p.rd_blk = row_descale_ld_block;
+    p.col8 = static_cast<uint8_t*>(d_col8_or_null); p.ld_col8 = ld_col8;
+    p.col_d = d_col_descale; p.cd_blk = col_descale_ld_block; p.cd_col = col_descale_ld_col;
+    return launch_quant<SRC_SWIGLU_GRAD>("cf_swiglu_backward_quantize_block128", p, is_e5m2, 2, as_stream(stream));
+}
+
+int cf_fp8_quantize_block128x128(const void* d_w, int ld_w, long long w_stride, int num_weights, int rows, int cols, void* d_out8,
+                                 int ld_out, long long out_stride, float* d_descale, long long descale_ld_row, long long descale_stride,
+                                 void* stream) {
+    const char* fn = "cf_fp8_quantize_block128x128";
+    CF_REQUIRE(num_weights >= 0 && rows >= 0 && cols >= 0, "%s: negative shape", fn);
+    if (num_weights == 0 || rows == 0 || cols == 0) return CF_OK;
+    CF_REQUIRE(d_w && d_out8 && d_descale, "%s: null pointer", fn);
+    CF_REQUIRE(ld_w >= cols && ld_out >= cols && descale_ld_row >= cdiv(cols, G), "%s: pitch smaller than a row", fn);
+    CF_REQUIRE(num_weights == 1 || (w_stride >= static_cast<long long>(rows - 1) * ld_w + cols &&
+                                    out_stride >= static_cast<long long>(rows - 1) * ld_out + cols &&
+                                    descale_stride >= (cdiv(rows, G) - 1) * descale_ld_row + cdiv(cols, G)),
+               "%s: matrices of the stack overlap", fn);
+    CF_REQUIRE(aligned(d_w, 2) && aligned(d_descale, 4), "%s: misaligned pointer", fn);
+    const int rc = require_sm100();
+    if (rc != CF_OK) return rc;
+    const int rb = static_cast<int>(cdiv(rows, G)), cb = static_cast<int>(cdiv(cols, G));
+    const long long blocks = static_cast<long long>(num_weights) * rb * cb;
+    if (blocks > 0x7fffffffll) { set_error("%s: too many blocks for one launch", fn); return CF_ERR_LIMIT; }
+    const int vec_in = aligned(d_w, 16) && ld_w % 8 == 0 && (num_weights == 1 || w_stride % 8 == 0);
+    const int vec_out = aligned(d_out8, 8) && ld_out % 8 == 0 && (num_weights == 1 || out_stride % 8 == 0);
+    k_quant_block128x128<<<static_cast<unsigned>(blocks), kWT, 0, as_stream(stream)>>>(
+        static_cast<const uint16_t*>(d_w), ld_w, w_stride, rows, cols, rb, cb, static_cast<uint8_t*>(d_out8), ld_out, out_stride,
+        d_descale, descale_ld_row, descale_stride, vec_in, vec_out);
+    CF_LAUNCH_CHECK("quant_block128x128");
+    return CF_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,935 @@
+// Block-scaled FP8 GEMM for sm_100a.
+//
+//   C[m,n] = sum over blocks b of 128 along K:  da[m,b] * db[n,b] * sum_{k in b} A8[m,k] * B8[n,k]
+//
+// The scale changes along the contraction, so one accumulator per output cannot take the whole sum: the tensor cores
+// multiply one block of 128 (four tcgen05.mma of 32) into a TMEM accumulator that starts from zero, and the epilogue
+// warps fold each finished block into fp32 registers, acc += (da db) * block, while the tensor cores fill the other TMEM
+// buffer with the next block. Both operands' scales are arbitrary fp32 numbers (no power-of-two restriction).
+//
+// Wide form (k_gemm_b128): tiles of 256 x 256 per CTA pair (cta_group::2) or 128 x 256 per CTA, persistent, 320 threads:
+//   warp 0      TMA producer (one elected lane)
+//   warp 1      TMEM allocator + MMA issuer (one elected lane)
+//   warps 2..9  promotion + epilogue: each owns 32 rows x 128 columns of the CTA's 128 x 256 tile in 128 registers a thread
+// Per block of 128 the MMAs of a CTA need 512 clocks; the promotion needs 64 packed multiply-adds per thread and two warps
+// per scheduler, 128 issue slots, and 128 KB of TMEM reads: it hides behind the MMAs.
+//
+// Narrow form (k_gemm_b128_narrow): few rows of A (tokens). The weights take the MMA's 128-row side and TN tokens its column
+// side, and the contraction is split over a cluster of CTAs whose partial sums meet in distributed shared memory, added in
+// rank order: every weight byte is read once, by enough CTAs to fill the chip, and no atomics are involved.
+//
+// Every wait on an mbarrier is bounded: a wait that gives up raises an abort flag, records a code in the context's status
+// word, drains the CTA's own copies and MMAs, frees TMEM and returns.
+#include "cf_common.cuh"
+#include "cf_internal.cuh"
+#include "cf_tc.cuh"
+
+namespace cf {
+
+int* ctx_status(cf_ctx* c);
+
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 128;                 // rows of A / C per CTA (TMEM lanes)
+constexpr int BN = 256;                 // output columns per tile
+constexpr int SB = 128;                 // elements of K that share a scale == BK
+constexpr int NUM_THREADS = 320;
+constexpr int EPI_WARPS = 8;
+constexpr int TMEM_COLS = 512;          // two 128x256 fp32 block sums per CTA
+constexpr int C_STAGING = EPI_WARPS * C_BOX_BYTES;
+
+template <bool PAIR>
+struct Cfg {
+    static constexpr int B_ROWS = PAIR ? 128 : 256;
+    static constexpr int STAGES = PAIR ? 6 : 4;
+    static constexpr int A_STAGE = BM * BK;
+    static constexpr int B_STAGE = B_ROWS * BK;
+    static constexpr int TILE_M = PAIR ? 256 : 128;
+    static constexpr int RING = STAGES * (A_STAGE + B_STAGE);
+    static constexpr int SMEM_BYTES = RING + C_STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+};
+
+enum OutKind { OUT_BF16 = 0, OUT_F32 = 1, OUT_F32_ADD = 2, OUT_BF16_ADD = 3 };
+
+struct Params {
+    int M = 0, N = 0, K = 0;                 // M: rows of C (grouped: rows of the compact buffers)
+    int groups = 0;                          // 0: dense
+    const int* d_counts = nullptr;
+    const int* d_offsets = nullptr;
+    const float* sa = nullptr;               // sa[row * sa_row + block * sa_blk]
+    long long sa_row = 0, sa_blk = 0;
+    const float* sb = nullptr;               // sb[(column / b_per) * sb_row + block * sb_blk + group * sb_group]
+    long long sb_row = 0, sb_blk = 0, sb_group = 0;
+    void* C = nullptr;
+    long long ldc = 0;
+    int out_kind = OUT_BF16;
+    int tma_out = 0;                         // full boxes leave through TMA
+    int a_mn = 0, b_mn = 0;                  // operand lies [K, rows] in memory
+    int a_e5m2 = 0, b_e5m2 = 0;
+    int raster_m = 8;
+    int* d_status = nullptr;
+};
+
+// ---- packed fp32 pairs ----------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ uint16_t to_bf16_bits(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+
+__device__ __forceinline__ void store_value(const Params& p, long long row, long long col, float v) {
+    const long long i = row * p.ldc + col;
+    if (p.out_kind == OUT_BF16) static_cast<uint16_t*>(p.C)[i] = to_bf16_bits(v);
+    else if (p.out_kind == OUT_F32) static_cast<float*>(p.C)[i] = v;
+    else if (p.out_kind == OUT_F32_ADD) static_cast<float*>(p.C)[i] += v;
+    else {
+        uint16_t* c = static_cast<uint16_t*>(p.C) + i;
+        *c = to_bf16_bits(bf16_bits_to_f32(*c) + v);
+    }
+}
+
+// ---- tiles ----------------------------------------------------------------------------------------------------------
+struct Tile {
+    int row0;        // first row of A / C
+    int end;         // rows [row0, end) belong to the tile's group
+    int n0;
+    int group;
+};
+
+// Rows of a group, cut to the buffer: counts and offsets are device data, and a row outside [0, M) is never touched.
+__device__ __forceinline__ void group_span(const Params& p, const int* counts, const int* offsets, int g, int& first, int& n) {
+    first = offsets[g];
+    n = counts[g];
+    if (first < 0 || first >= p.M || n < 0) { n = 0; first = 0; }
+    n = min(n, p.M - first);
+}
+__device__ __forceinline__ int row_blocks(const Params& p, const int* counts, const int* offsets, int TM) {
+    if (p.groups == 0) return (p.M + TM - 1) / TM;
+    int t = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        int first, n;
+        group_span(p, counts, offsets, g, first, n);
+        t += (n + TM - 1) / TM;
+    }
+    return t;
+}
+// Bands of raster_m row blocks: consecutive tiles walk down a band, then one column block right, so the tiles in flight
+// share few slabs of A and B.
+__device__ __forceinline__ Tile tile_at(const Params& p, const int* counts, const int* offsets, int tile, int m_blocks, int TM) {
+    Tile t;
+    const int n_blocks = (p.N + BN - 1) / BN;
+    const int band_tiles = p.raster_m * n_blocks;
+    const int band = tile / band_tiles;
+    const int first_m = band * p.raster_m;
+    const int band_m = min(p.raster_m, m_blocks - first_m);
+    const int r = tile - band * band_tiles;
+    const int nb = r / band_m;
+    int mb = first_m + (r - nb * band_m);
+    t.n0 = nb * BN;
+    if (p.groups == 0) {
+        t.group = 0;
+        t.row0 = mb * TM;
+        t.end = p.M;
+        return t;
+    }
+    int g = 0, first = 0, n = 0;
+    for (; g < p.groups; ++g) {
+        group_span(p, counts, offsets, g, first, n);
+        const int blocks = (n + TM - 1) / TM;
+        if (mb < blocks) break;
+        mb -= blocks;
+    }
+    t.group = g;
+    t.row0 = first + mb * TM;
+    t.end = first + n;
+    return t;
+}
+
+constexpr int kGroupsInSmem = 128;
+
+// BVEC: db has one value per column of C and block (b_per = 1); otherwise one per 128 columns and block.
+template <bool PAIR, bool BVEC>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ CUtensorMap map_c, const Params p) {
+    using C = Cfg<PAIR>;
+    constexpr int STAGES = C::STAGES, A_STAGE = C::A_STAGE, B_STAGE = C::B_STAGE, TM = C::TILE_M;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const uint32_t smem_a = base;
+    const uint32_t smem_b = base + STAGES * A_STAGE;
+    const uint32_t smem_c = smem_b + STAGES * B_STAGE;
+    const uint32_t bars = smem_c + C_STAGING;
+    const uint32_t full_bar = bars, empty_bar = bars + 8 * STAGES;
+    const uint32_t tfull_bar = bars + 16 * STAGES, tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16;
+    uint8_t* gen = smem_raw + (base - raw);
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C_STAGING + 16 * STAGES + 48);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(const_cast<uint32_t*>(s_tmem) + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cta_rank = PAIR ? cluster_ctarank() : 0u;
+    const bool leader = cta_rank == 0;
+    const int unit = PAIR ? (blockIdx.x >> 1) : blockIdx.x;
+    const int n_units = PAIR ? (gridDim.x >> 1) : gridDim.x;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full_bar + 8 * s, 1);
+            mbar_init(empty_bar + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar + 8 * a, 1);
+            mbar_init(tempty_bar + 8 * a, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+        }
+        mbar_init(drain_bar, 1);
+        s_abort[0] = 0;
+        s_abort[1] = 0;                                      // stays 0: abort source for the drain waits
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        if (p.tma_out) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(s_tmem))), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(s_tmem))), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync_all();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *s_tmem;
+    pdl_wait();                                              // everything above touched only this CTA's own memory
+
+    __shared__ int s_groups[2 * kGroupsInSmem];
+    const int* counts = p.d_counts;
+    const int* offsets = p.d_offsets;
+    if (p.groups > 0 && p.groups <= kGroupsInSmem) {         // the tile mapping walks them for every tile
+        for (int e = threadIdx.x; e < p.groups; e += NUM_THREADS) {
+            s_groups[e] = p.d_counts[e];
+            s_groups[kGroupsInSmem + e] = p.d_offsets[e];
+        }
+        __syncthreads();
+        counts = s_groups;
+        offsets = s_groups + kGroupsInSmem;
+    }
+    const int m_blocks = row_blocks(p, counts, offsets, TM);
+    const int total_tiles = m_blocks * ((p.N + BN - 1) / BN);
+    const int k_iters = (p.K + BK - 1) / BK;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer (both CTAs of a pair)
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            const uint32_t full_dst = PAIR ? mapa(full_bar, 0) : full_bar;
+            for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
+                const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
+                const int a_row = tc_.row0 + static_cast<int>(cta_rank) * BM;
+                const int b_col = tc_.n0 + static_cast<int>(cta_rank) * C::B_ROWS;       // rank is 0 in the single form
+                for (int kb = 0; kb < k_iters; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(empty_bar + 8 * s, ((it / STAGES) & 1) ^ 1, s_abort)) { ok = false; break; }
+                    // K-major operand: x runs along K. MN-major operand ([K, rows] in memory): x runs along the rows, the
+                    // box rows are K (pair form only: a CTA's share is one box of 128 bytes)
+                    const int ax = p.a_mn ? a_row : kb * BK, ay = p.a_mn ? kb * BK : a_row;
+                    const int bx = p.b_mn ? b_col : kb * BK, by = p.b_mn ? kb * BK : tc_.group * p.N + b_col;
+                    if (PAIR) {
+                        if (leader) mbar_expect_tx(full_bar + 8 * s, 2 * (A_STAGE + B_STAGE));
+                        tma_load_2d_pair(smem_a + s * A_STAGE, &map_a, full_dst + 8 * s, ax, ay);
+                        tma_load_2d_pair(smem_b + s * B_STAGE, &map_b, full_dst + 8 * s, bx, by);
+                    } else {
+                        mbar_expect_tx(full_bar + 8 * s, A_STAGE + B_STAGE);
+                        tma_load_2d(smem_a + s * A_STAGE, &map_a, full_bar + 8 * s, ax, ay);
+                        tma_load_2d(smem_b + s * B_STAGE, &map_b, full_bar + 8 * s, bx, by);
+                    }
+                }
+            }
+            if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x500 | 1); }
+            if ((*s_abort || !ok) && leader) {
+                for (int j = max(0, it - STAGES); j < it; ++j)
+                    mbar_wait(full_bar + 8 * (j % STAGES), (j / STAGES) & 1, s_abort + 1 /*never set*/, DRAIN_NS);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer (leader CTA only)
+        if (lane == 0 && leader) {
+            const uint32_t idesc = make_idesc(p.a_e5m2, p.b_e5m2, TM, BN, p.a_mn, p.b_mn);
+            // one MMA covers 32 of K: 32 bytes further inside the swizzle atom of a K-major operand, 32 rows of 128 bytes
+            // further in an MN-major one
+            const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
+            int it = 0;
+            bool ok = true;
+            for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
+                for (int kb = 0; kb < k_iters; ++kb, ++it) {
+                    const int s = it % STAGES, buf = it & 1;
+                    if (!mbar_wait(tempty_bar + 8 * buf, ((it >> 1) & 1) ^ 1, s_abort)) { ok = false; break; }
+                    if (!mbar_wait(full_bar + 8 * s, (it / STAGES) & 1, s_abort)) { ok = false; break; }
+                    tcgen05_fence_after();
+                    const uint64_t adesc = make_smem_desc(smem_a + s * A_STAGE);
+                    const uint64_t bdesc = make_smem_desc(smem_b + s * B_STAGE);
+                    const uint32_t tmem_d = tmem_base + buf * BN;
+#pragma unroll
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                        else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                    }
+                    if (PAIR) {
+                        tcgen05_commit_pair(empty_bar + 8 * s);
+                        tcgen05_commit_pair(tfull_bar + 8 * buf);
+                    } else {
+                        tcgen05_commit(empty_bar + 8 * s);
+                        tcgen05_commit(tfull_bar + 8 * buf);
+                    }
+                }
+            }
+            if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x600 | 1); }
+            if (*s_abort || !ok) {
+                if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar) : "memory");
+                else tcgen05_commit(drain_bar);
+                mbar_wait(drain_bar, 0, s_abort + 1, DRAIN_NS);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ promotion + epilogue (both CTAs of a pair)
+        const int quarter = warp & 3;                      // TMEM lanes this warp may read
+        const int half = (warp - 2) >> 2;                  // which 128 columns of the tile
+        const uint32_t tempty_dst = PAIR ? mapa(tempty_bar, 0) : tempty_bar;
+        const uint32_t box = smem_c + static_cast<uint32_t>(warp - 2) * C_BOX_BYTES;
+        float* box_f = reinterpret_cast<float*>(gen + C::RING + (warp - 2) * C_BOX_BYTES);
+        const uint64_t store_policy = l2_policy_evict_first();
+        int it = 0;
+        bool ok = true;
+        for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
+            const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
+            const int warp_row = tc_.row0 + static_cast<int>(cta_rank) * BM + quarter * 32;
+            const int row = warp_row + lane;
+            const int wcol = tc_.n0 + half * 128;          // first column of this warp
+            const bool live = row < tc_.end;
+            const float* sa = p.sa + (live ? row * p.sa_row : 0);
+            const float* sb = p.sb + tc_.group * p.sb_group;
+            // columns of this warp beyond N get scale 0 (their products are never stored)
+            if (!BVEC) sb += (wcol / SB) * p.sb_row;
+            const bool sb_ok = wcol < p.N;
+            uint64_t acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) acc[j] = 0ull;
+            float sa_next = live ? __ldg(sa) : 0.0f;
+            float sb_next = 0.0f;
+            float cs[4];                                   // BVEC: lane l carries columns l, l+32, l+64, l+96 of the next block
+            if (BVEC) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = wcol + lane + 32 * q;
+                    cs[q] = c < p.N ? __ldg(sb + c * p.sb_row) : 0.0f;
+                }
+                if (lane == 0) bulk_wait_read_0();         // the box doubles as the scales' buffer: its last store has left
+                __syncwarp();
+            } else {
+                sb_next = sb_ok ? __ldg(sb) : 0.0f;
+            }
+            for (int kb = 0; kb < k_iters; ++kb, ++it) {
+                const int buf = it & 1;
+                const float s_row = BVEC ? sa_next : sa_next * sb_next;
+                if (BVEC) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) box_f[buf * 128 + lane + 32 * q] = cs[q];
+                    __syncwarp();
+                }
+                if (kb + 1 < k_iters) {                    // the next block's scales are on their way during this one
+                    if (live) sa_next = __ldg(sa + (kb + 1) * p.sa_blk);
+                    if (BVEC) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int c = wcol + lane + 32 * q;
+                            if (c < p.N) cs[q] = __ldg(sb + c * p.sb_row + (kb + 1) * p.sb_blk);
+                        }
+                    } else if (sb_ok) {
+                        sb_next = __ldg(sb + (kb + 1) * p.sb_blk);
+                    }
+                }
+                if (!mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort)) { ok = false; break; }
+                tcgen05_fence_after();
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
+                const uint64_t s2 = pack_f2(s_row, s_row);
+                uint32_t v[2][16];
+                tmem_ld16(taddr, v[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    tmem_ld_wait();
+                    if (c < 7) tmem_ld16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint64_t x = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
+                        if (BVEC) {
+                            const float2 b2 = *reinterpret_cast<const float2*>(box_f + buf * 128 + c * 16 + 2 * j);
+                            x = mul_f2(x, pack_f2(b2.x, b2.y));
+                        }
+                        acc[c * 8 + j] = fma_f2(x, s2, acc[c * 8 + j]);
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster(tempty_dst + 8 * buf); else mbar_arrive(tempty_bar + 8 * buf);
+                }
+            }
+            if (!ok) break;
+            // ---- the tile's 32 rows x 128 columns of this warp leave
+            const bool f32 = p.out_kind == OUT_F32 || p.out_kind == OUT_F32_ADD;
+            // a box may only leave whole: in the ragged form its rows must all belong to the group
+            const bool boxes = p.tma_out && warp_row < tc_.end && (p.groups == 0 || warp_row + 32 <= tc_.end);
+            const uint32_t row_off = static_cast<uint32_t>(lane) * 128u;
+            const uint32_t sw = static_cast<uint32_t>(lane & 7);
+            if (lane == 0) bulk_wait_read_0();
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {                  // 32 columns at a time
+                const int col0 = wcol + c * 32;
+                const int width = f32 ? 32 : 64;
+                const int box_col = f32 ? col0 : wcol + (c >> 1) * 64;
+                if (col0 < p.N) {                          // warp-uniform
+                    if (boxes && box_col + width <= p.N) {
+                        if (f32 ? c > 0 : c == 2) {        // the previous box has left this buffer
+                            if (lane == 0) bulk_wait_read_0();
+                            __syncwarp();
+                        }
+                        if (f32) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {  // 16-byte chunk q of a row sits at q ^ (row % 8): 128B swizzle
+                                float f[4];
+                                unpack_f2(acc[c * 16 + 2 * q], f[0], f[1]);
+                                unpack_f2(acc[c * 16 + 2 * q + 1], f[2], f[3]);
+                                st_shared_v4(box + row_off + ((static_cast<uint32_t>(q) ^ sw) << 4), __float_as_uint(f[0]),
+                                             __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                            }
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    float lo, hi;
+                                    unpack_f2(acc[c * 16 + 4 * q + e], lo, hi);
+                                    w[e] = pack_bf16x2(lo, hi);
+                                }
+                                st_shared_v4(box + row_off + ((static_cast<uint32_t>((c & 1) * 4 + q) ^ sw) << 4), w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                        if (f32 || (c & 1)) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (p.out_kind == OUT_F32_ADD) tma_reduce_add_2d(&map_c, box, box_col, warp_row);
+                                else tma_store_2d(&map_c, box, box_col, warp_row, store_policy);
+                                bulk_commit();
+                            }
+                        }
+                    } else {
+                        // edges, ragged rows, unaligned or accumulated bf16 outputs: the 32 x 32 values turn around in the
+                        // box, so that a warp writes 32 neighbouring columns of one row at a time
+                        if (lane == 0) bulk_wait_read_0();
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            float lo, hi;
+                            unpack_f2(acc[c * 16 + j], lo, hi);
+                            box_f[lane * 32 + ((2 * j) ^ lane)] = lo;
+                            box_f[lane * 32 + ((2 * j + 1) ^ lane)] = hi;
+                        }
+                        __syncwarp();
+                        const int rows = min(32, tc_.end - warp_row);
+                        for (int r = 0; r < rows; ++r)
+                            if (col0 + lane < p.N) store_value(p, warp_row + r, col0 + lane, box_f[r * 32 + (lane ^ r)]);
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+        if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x700 | 1); }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync_all();          // the peer may still read this CTA's operands / signal its barriers
+    if (warp == 1) {
+        __syncwarp();
+        tcgen05_fence_after();
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// ------------------------------------------------------------------ narrow form
+constexpr int NARROW_THREADS = 192;        // warp 0 producer, warp 1 MMA issuer, warps 2..5 promotion
+template <int TN>
+struct Narrow {
+    static constexpr int W_STAGE = 128 * BK;
+    static constexpr int X_STAGE = TN * BK;
+    static constexpr int STAGES = TN <= 32 ? 5 : 4;
+    static constexpr int RING = STAGES * (W_STAGE + X_STAGE);
+    static constexpr int SCALES = 4 * 2 * TN * 4;          // per promotion warp two copies of a block's token scales
+    static constexpr int TMEM = 2 * TN < 32 ? 32 : 2 * TN;
+    static constexpr int PARTIAL = TN * 128 * 4;           // overlays the ring after the last block
+    static constexpr int SMEM_BYTES = RING + SCALES + 1024 + 256;
+    static_assert(PARTIAL <= RING, "partial sums overlay the ring");
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// map_w: weights [N, K]; map_x: tokens [M, K]. Grid: x = n tile * splits + rank in the cluster, y = token tile.
+template <int TN>
+__global__ void __launch_bounds__(NARROW_THREADS)
+k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p, int splits, int b_per) {
+    using C = Narrow<TN>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - raw);
+    const uint32_t smem_w = base, smem_x = base + STAGES * C::W_STAGE;
+    float* s_scales = reinterpret_cast<float*>(gen + C::RING);
+    const uint32_t bars = base + C::RING + C::SCALES;
+    const uint32_t full_bar = bars, empty_bar = bars + 8 * STAGES, tfull_bar = bars + 16 * STAGES, tempty_bar = tfull_bar + 16,
+                   drain_bar = tempty_bar + 16;
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C::SCALES + 16 * STAGES + 48);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(const_cast<uint32_t*>(s_tmem) + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % splits;
+    const int n0 = (blockIdx.x / splits) * 128;
+    const int m0 = blockIdx.y * TN;
+    const int k_iters = (p.K + BK - 1) / BK;
+    const int kb0 = static_cast<int>(static_cast<long long>(k_iters) * rank / splits);
+    const int kb1 = static_cast<int>(static_cast<long long>(k_iters) * (rank + 1) / splits);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full_bar + 8 * s, 1);
+            mbar_init(empty_bar + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar + 8 * a, 1);
+            mbar_init(tempty_bar + 8 * a, 4);
+        }
+        mbar_init(drain_bar, 1);
+        s_abort[0] = 0;
+        s_abort[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(s_tmem))), "r"(C::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *s_tmem;
+    pdl_wait();
+
+    float acc[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[j] = 0.0f;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            int it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!mbar_wait(empty_bar + 8 * s, ((it / STAGES) & 1) ^ 1, s_abort)) { ok = false; break; }
+                mbar_expect_tx(full_bar + 8 * s, C::W_STAGE + C::X_STAGE);
+                tma_load_2d(smem_w + s * C::W_STAGE, &map_w, full_bar + 8 * s, kb * BK, n0);
+                tma_load_2d(smem_x + s * C::X_STAGE, &map_x, full_bar + 8 * s, kb * BK, m0);
+            }
+            if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x800 | 1); }
+            if (*s_abort || !ok)
+                for (int j = max(0, it - STAGES); j < it; ++j)
+                    mbar_wait(full_bar + 8 * (j % STAGES), (j / STAGES) & 1, s_abort + 1, DRAIN_NS);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = make_idesc(p.b_e5m2, p.a_e5m2, 128, TN, 0, 0);
+            bool ok = true;
+            int it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES, buf = it & 1;
+                if (!mbar_wait(tempty_bar + 8 * buf, ((it >> 1) & 1) ^ 1, s_abort)) { ok = false; break; }
+                if (!mbar_wait(full_bar + 8 * s, (it / STAGES) & 1, s_abort)) { ok = false; break; }
+                tcgen05_fence_after();
+                const uint64_t wdesc = make_smem_desc(smem_w + s * C::W_STAGE);
+                const uint64_t xdesc = make_smem_desc(smem_x + s * C::X_STAGE);
+#pragma unroll
+                for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                    umma_f8(tmem_base + buf * TN, wdesc + 2 * kk, xdesc + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                tcgen05_commit(empty_bar + 8 * s);
+                tcgen05_commit(tfull_bar + 8 * buf);
+            }
+            if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x900 | 1); }
+            if (*s_abort || !ok) {
+                tcgen05_commit(drain_bar);
+                mbar_wait(drain_bar, 0, s_abort + 1, DRAIN_NS);
+            }
+        }
+    } else {
+        // lane = output feature n, TMEM column = token
+        const int quarter = warp & 3;
+        const int n = n0 + quarter * 32 + lane;
+        const bool n_ok = n < p.N;
+        const float* sw = p.sb + (n_ok ? (n / b_per) * p.sb_row : 0);
+        float* sc = s_scales + (warp - 2) * 2 * TN;
+        constexpr int PER = (TN + 31) / 32;
+        float xs[PER];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int m = lane + 32 * q;
+            xs[q] = (m < TN && m0 + m < p.M && kb0 < kb1) ? __ldg(p.sa + (m0 + m) * p.sa_row + kb0 * p.sa_blk) : 0.0f;
+        }
+        float w_next = n_ok && kb0 < kb1 ? __ldg(sw + kb0 * p.sb_blk) : 0.0f;
+        bool ok = true;
+        int it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int buf = it & 1;
+#pragma unroll
+            for (int q = 0; q < PER; ++q)
+                if (lane + 32 * q < TN) sc[buf * TN + lane + 32 * q] = xs[q];
+            __syncwarp();
+            const float w = w_next;
+            if (kb + 1 < kb1) {
+                if (n_ok) w_next = __ldg(sw + (kb + 1) * p.sb_blk);
+#pragma unroll
+                for (int q = 0; q < PER; ++q) {
+                    const int m = lane + 32 * q;
+                    if (m < TN && m0 + m < p.M) xs[q] = __ldg(p.sa + (m0 + m) * p.sa_row + (kb + 1) * p.sa_blk);
+                }
+            }
+            if (!mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
+#pragma unroll
+            for (int c = 0; c < TN / 16; ++c) {
+                uint32_t v[16];
+                tmem_ld16(taddr + c * 16, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[j]) * w, sc[buf * TN + c * 16 + j], acc[c * 16 + j]);
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty_bar + 8 * buf);
+        }
+        if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xa00 | 1); }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();                       // every block of this CTA has been consumed: the ring is free
+    if (warp == 1) {
+        __syncwarp();
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM) : "memory");
+    }
+    if (splits == 1) {
+        if (warp >= 2) {
+            const int n = n0 + (warp & 3) * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+                if (n < p.N && m0 + t < p.M) store_value(p, m0 + t, n, acc[t]);
+        }
+        return;
+    }
+    float* part = reinterpret_cast<float*>(gen);                 // [TN][128]
+    if (warp >= 2) {
+        const int f = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < TN; ++t) part[t * 128 + f] = acc[t];
+    }
+    cluster_sync_all();
+    if (warp >= 2) {
+        // this CTA adds up the tokens rank, rank + splits, ...: partial sums in rank order
+        const int f = (warp & 3) * 32 + lane;
+        for (int t = rank; t < TN && m0 + t < p.M; t += splits) {
+            float v = 0.0f;
+            for (int r = 0; r < splits; ++r) v += ld_cluster_f32(mapa(base + (t * 128 + f) * 4, r));
+            if (n0 + f < p.N) store_value(p, m0 + t, n0 + f, v);
+        }
+    }
+    cluster_sync_all();                                          // the others have read this CTA's sums
+}
+
+// ------------------------------------------------------------------ host side
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+
+template <bool PAIR>
+int set_smem() {
+    cudaError_t e = cudaFuncSetAttribute(k_gemm_b128<PAIR, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_gemm_b128<PAIR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES);
+    return e == cudaSuccess ? CF_OK : cuda_fail(e, "cudaFuncSetAttribute(k_gemm_b128)");
+}
+
+// CTA pairs the current device keeps resident at once, asked once per device.
+int resident_pairs(int* pairs) {
+    static std::mutex mu;
+    static int cached[64];                  // 0 unknown, else pairs + 1
+    int dev = 0;
+    CF_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    int& c = cached[dev & 63];
+    if (c == 0) {
+        int rc = set_smem<true>();
+        if (rc == CF_OK) rc = set_smem<false>();
+        if (rc != CF_OK) return rc;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * sm_count());
+        cfg.blockDim = dim3(NUM_THREADS);
+        cfg.dynamicSmemBytes = Cfg<true>::SMEM_BYTES;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        CF_CUDA(cudaOccupancyMaxActiveClusters(&n, k_gemm_b128<true, true>, &cfg));
+        if (n < 1) { set_error("no CTA pair fits this device"); return CF_ERR_UNSUPPORTED; }
+        c = n + 1;
+    }
+    *pairs = c - 1;
+    return CF_OK;
+}
+
+template <int TN>
+int launch_narrow(const CUtensorMap& map_w, const CUtensorMap& map_x, const Params& p, int splits, int b_per, cudaStream_t st) {
+    using C = Narrow<TN>;
+    static std::once_flag once[64];
+    int dev = 0;
+    CF_CUDA(cudaGetDevice(&dev));
+    cudaError_t e = cudaSuccess;
+    std::call_once(once[dev & 63], [&] { e = cudaFuncSetAttribute(k_gemm_b128_narrow<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES); });
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(k_gemm_b128_narrow)");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(cdiv(p.N, 128) * splits), static_cast<unsigned>(cdiv(p.M, TN)));
+    cfg.blockDim = dim3(NARROW_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128_narrow<TN>, map_w, map_x, p, splits, b_per));
+    CF_LAUNCH_CHECK("gemm_b128_narrow");
+    return CF_OK;
+}
+
+// a_rows_mem / b_rows_mem: row extents of the two byte matrices in memory. b_per: columns of C per B scale (128 or 1).
+int launch_b128(const char* fn, const void* A, long long lda, const void* B, long long ldb, long long b_rows_mem, Params p, int b_per,
+                cudaStream_t st) {
+    if (!aligned(A, 16) || !aligned(B, 16) || lda % 16 != 0 || ldb % 16 != 0) {
+        set_error("%s: the FP8 operands need 16-byte aligned bases and row pitches", fn);
+        return CF_ERR_UNSUPPORTED;
+    }
+    int rc = require_sm100();
+    if (rc != CF_OK) return rc;
+    CUtensorMap map_a, map_b, map_c;
+    // Few rows of a K-major product: the narrow form
+    if (p.groups == 0 && !p.a_mn && !p.b_mn && p.M <= 128) {
+        const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+        const long long ctas = cdiv(p.N, 128) * cdiv(p.M, tn);
+        const int k_iters = static_cast<int>(cdiv(p.K, BK));
+        int splits = 1;
+        while (splits < 8 && ctas * splits * 2 <= 2ll * sm_count() && k_iters >= 4 * splits) splits *= 2;
+        rc = make_map(&map_b, B, b_rows_mem, p.K, ldb, 128);
+        if (rc == CF_OK) rc = make_map(&map_a, A, p.M, p.K, lda, tn);
+        if (rc != CF_OK) return rc;
+        if (tn == 16) return launch_narrow<16>(map_b, map_a, p, splits, b_per, st);
+        if (tn == 32) return launch_narrow<32>(map_b, map_a, p, splits, b_per, st);
+        if (tn == 64) return launch_narrow<64>(map_b, map_a, p, splits, b_per, st);
+        return launch_narrow<128>(map_b, map_a, p, splits, b_per, st);
+    }
+    int pairs = 0;
+    rc = resident_pairs(&pairs);
+    if (rc != CF_OK) return rc;
+    const long long rows_per_group = p.groups > 0 ? p.M / p.groups : p.M;
+    const bool pair = p.a_mn || p.b_mn || rows_per_group >= 512;
+    rc = p.a_mn ? make_map(&map_a, A, p.K, p.M, lda, BK) : make_map(&map_a, A, p.M, p.K, lda, BM);
+    if (rc == CF_OK) rc = p.b_mn ? make_map(&map_b, B, b_rows_mem, p.N, ldb, BK) : make_map(&map_b, B, b_rows_mem, p.K, ldb, pair ? 128 : 256);
+    if (rc != CF_OK) return rc;
+    const bool f32 = p.out_kind == OUT_F32 || p.out_kind == OUT_F32_ADD;
+    p.tma_out = p.out_kind != OUT_BF16_ADD && aligned(p.C, 16) && p.ldc % (f32 ? 4 : 8) == 0 && p.N >= (f32 ? 32 : 64);
+    if (p.tma_out) {
+        rc = f32 ? make_map_c_f32(&map_c, p.C, p.M, p.N, p.ldc) : make_map_c(&map_c, p.C, p.M, p.N, p.ldc);
+        if (rc != CF_OK) return rc;
+    } else {
+        map_c = map_a;                      // not read by the kernel
+    }
+    const int tm = pair ? 256 : 128;
+    const long long tiles = (cdiv(p.M, tm) + p.groups) * cdiv(p.N, BN);
+    if (tiles > 0x3fffffffll) { set_error("%s: product too large", fn); return CF_ERR_LIMIT; }
+    const long long most = pair ? pairs : sm_count();
+    const int units = static_cast<int>(tiles < most ? tiles : most);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pair ? 2 * units : units);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = pair ? Cfg<true>::SMEM_BYTES : Cfg<false>::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pair ? 2 : 1;
+    if (pair && b_per == 1) CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128<true, true>, map_a, map_b, map_c, p));
+    else if (pair) CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128<true, false>, map_a, map_b, map_c, p));
+    else if (b_per == 1) CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128<false, true>, map_a, map_b, map_c, p));
+    else CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128<false, false>, map_a, map_b, map_c, p));
+    CF_LAUNCH_CHECK("gemm_b128");
+    return CF_OK;
+}
+
+int out_kind(int out_fp32, int accumulate) {
+    return out_fp32 ? (accumulate ? OUT_F32_ADD : OUT_F32) : (accumulate ? OUT_BF16_ADD : OUT_BF16);
+}
+
+// What every form checks. Rows of A: M x K (or K x M), of B: N x K (or K x N).
+int check_common(const char* fn, cf_ctx* ctx, int M, int N, int K, const void* A, const void* sa, const void* B, const void* sb,
+                 const void* C, long long ldc, int fp32) {
+    CF_REQUIRE(ctx != nullptr, "%s: null context", fn);
+    CF_REQUIRE(M >= 0 && N >= 0 && K >= 0, "%s: negative shape", fn);
+    if (M == 0 || N == 0) return CF_OK;
+    CF_REQUIRE(K > 0, "%s: an empty contraction is not supported", fn);
+    CF_REQUIRE(A && B && C, "%s: null matrix pointer", fn);
+    CF_REQUIRE(sa && sb, "%s: null descale pointer", fn);
+    CF_REQUIRE(ldc >= N, "%s: output pitch smaller than a row", fn);
+    CF_REQUIRE(aligned(sa, 4) && aligned(sb, 4) && aligned(C, fp32 ? 4 : 2), "%s: misaligned pointer", fn);
+    return CF_OK;
+}
+
+}  // namespace
+}  // namespace cf
+
+using namespace cf;
+
+extern "C" {
+
+int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                            long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb, const float* d_b_descale,
+                            long long b_descale_ld_row, long long b_descale_ld_block, int b_rows_per_scale, void* d_C, int ldc,
+                            int out_fp32, int accumulate, void* stream) {
+    const char* fn = "cf_gemm_fp8_block128_nt";
+    const int rc = check_common(fn, ctx, M, N, K, d_A, d_a_descale, d_B, d_b_descale, d_C, ldc, out_fp32);
+    if (rc != CF_OK || M == 0 || N == 0) return rc;
+    CF_REQUIRE(lda >= K && ldb >= K, "%s: operand pitch smaller than a row", fn);
+    CF_REQUIRE(b_rows_per_scale == 128 || b_rows_per_scale == 1, "%s: a scale of B covers 128 rows or 1", fn);
+    Params p;
+    p.M = M; p.N = N; p.K = K;
+    p.sa = d_a_descale; p.sa_row = a_descale_ld_row; p.sa_blk = a_descale_ld_block;
+    p.sb = d_b_descale; p.sb_row = b_descale_ld_row; p.sb_blk = b_descale_ld_block;
+    p.C = d_C; p.ldc = ldc; p.out_kind = out_kind(out_fp32, accumulate);
+    p.a_e5m2 = a_is_e5m2 ? 1 : 0;
+    p.d_status = ctx_status(ctx);
+    return launch_b128(fn, d_A, lda, d_B, ldb, N, p, b_rows_per_scale, as_stream(stream));
+}
+
+int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_rows, int N, int K, const int* d_counts,
+                                    const int* d_offsets, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                                    long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb,
+                                    const float* d_b_descale, long long b_descale_ld_row, long long b_descale_stride, void* d_C, int ldc,
+                                    void* stream) {
+    const char* fn = "cf_gemm_fp8_block128_nt_grouped";
+    const int rc = check_common(fn, ctx, max_total_rows, N, K, d_A, d_a_descale, d_B, d_b_descale, d_C, ldc, 0);
+    if (rc != CF_OK || max_total_rows == 0 || N == 0) return rc;
+    CF_REQUIRE(num_experts > 0 && d_counts && d_offsets, "%s: no groups", fn);
+    CF_REQUIRE(aligned(d_counts, 4) && aligned(d_offsets, 4), "%s: misaligned pointer", fn);
+    CF_REQUIRE(lda >= K && ldb >= K, "%s: operand pitch smaller than a row", fn);
+    if (static_cast<long long>(num_experts) * N > 0x7fffffffll) { set_error("%s: more than 2^31 weight rows", fn); return CF_ERR_LIMIT; }
+    Params p;
+    p.M = max_total_rows; p.N = N; p.K = K;
+    p.groups = num_experts; p.d_counts = d_counts; p.d_offsets = d_offsets;
+    p.sa = d_a_descale; p.sa_row = a_descale_ld_row; p.sa_blk = a_descale_ld_block;
+    p.sb = d_b_descale; p.sb_row = b_descale_ld_row; p.sb_blk = 1; p.sb_group = b_descale_stride;
+    p.C = d_C; p.ldc = ldc; p.out_kind = OUT_BF16;
+    p.a_e5m2 = a_is_e5m2 ? 1 : 0;
+    p.d_status = ctx_status(ctx);
+    return launch_b128(fn, d_A, lda, d_B, ldb, static_cast<long long>(num_experts) * N, p, 128, as_stream(stream));
+}
+
+int cf_gemm_fp8_block128_nn(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                            long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B_kn, int ldb,
+                            const float* d_b_descale, long long b_descale_ld_row, void* d_C, int ldc, int out_fp32, int accumulate,
+                            void* stream) {
+    const char* fn = "cf_gemm_fp8_block128_nn";
+    const int rc = check_common(fn, ctx, M, N, K, d_A, d_a_descale, d_B_kn, d_b_descale, d_C, ldc, out_fp32);
+    if (rc != CF_OK || M == 0 || N == 0) return rc;
+    CF_REQUIRE(lda >= K && ldb >= N, "%s: operand pitch smaller than a row", fn);
+    Params p;
+    p.M = M; p.N = N; p.K = K;
+    p.sa = d_a_descale; p.sa_row = a_descale_ld_row; p.sa_blk = a_descale_ld_block;
+    p.sb = d_b_descale; p.sb_row = 1; p.sb_blk = b_descale_ld_row;      // scales lie [K / 128, N / 128], like the blocks of B
+    p.C = d_C; p.ldc = ldc; p.out_kind = out_kind(out_fp32, accumulate);
+    p.a_e5m2 = a_is_e5m2 ? 1 : 0;
+    p.b_mn = 1;
+    p.d_status = ctx_status(ctx);
+    return launch_b128(fn, d_A, lda, d_B_kn, ldb, K, p, 128, as_stream(stream));
+}
+
+int cf_gemm_fp8_block128_dw(cf_ctx* ctx, int M, int N, int K, const void* d_X, int ldx, int x_is_e5m2, const float* d_x_descale,
+                            long long x_descale_ld_block, long long x_descale_ld_col, const void* d_dY, int ldy, int dy_is_e5m2,
+                            const float* d_dy_descale, long long dy_descale_ld_block, long long dy_descale_ld_col, void* d_dW, int ldc,
+                            int out_fp32, int accumulate, void* stream) {
+    const char* fn = "cf_gemm_fp8_block128_dw";
+    const int rc = check_common(fn, ctx, M, N, K, d_X, d_x_descale, d_dY, d_dy_descale, d_dW, ldc, out_fp32);
+    if (rc != CF_OK || M == 0 || N == 0) return rc;
+    CF_REQUIRE(ldx >= M && ldy >= N, "%s: operand pitch smaller than a row", fn);
+    Params p;
+    p.M = M; p.N = N; p.K = K;
+    p.sa = d_x_descale; p.sa_row = x_descale_ld_col; p.sa_blk = x_descale_ld_block;
+    p.sb = d_dy_descale; p.sb_row = dy_descale_ld_col; p.sb_blk = dy_descale_ld_block;
+    p.C = d_dW; p.ldc = ldc; p.out_kind = out_kind(out_fp32, accumulate);
+    p.a_e5m2 = x_is_e5m2 ? 1 : 0;
+    p.b_e5m2 = dy_is_e5m2 ? 1 : 0;
+    p.a_mn = p.b_mn = 1;
+    p.d_status = ctx_status(ctx);
+    return launch_b128(fn, d_X, ldx, d_dY, ldy, K, p, 1, as_stream(stream));
+}
+
+}  // extern "C"

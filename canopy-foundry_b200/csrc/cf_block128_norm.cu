@@ -1,0 +1,374 @@
+// Residual addition + RMS norm with block-scaled FP8 output, and the gradient of the pair.
+//
+//   forward   h = bf16(x + residual);  rms = sqrt(mean(h^2) + eps);  y = (h / rms) * scale
+//             per 128 values of y: a = max(max|y|, 1e-12), descale = a / 448, code = e4m3(y * (448 / a))
+//   backward  u = dy * scale;  dx = (u - h * sum(u h) / (H rms^2)) / rms + dh;  dscale = sum over rows of dy * h / rms
+//
+// h is rounded to bf16 before the norm reads it: it is the residual stream the next layers and the backward pass see. y is
+// NOT rounded to bf16 on its way to the codes (one rounding, descales from fp32); the optional bf16 copy of y is.
+// Sums, rms and descales are fp32.
+//
+// Both are streams: forward 2+2 B in, 2+1 B out per element (7), backward 2+2+2 in, 2 out (8). A row lives in the registers
+// of one block between its reduction and its second use, 16 neighbouring threads hold one group of 128, and one block
+// barrier per row joins the row sum (two copies of the partial sums alternate, so the next row needs no second barrier).
+// The gain's gradient is summed per block over the block's rows in registers, written as one partial row per block and
+// added up in block order by a second launch: no atomics, so the result does not depend on timing.
+#include "cf_common.cuh"
+#include "cf_internal.cuh"
+
+namespace cf {
+namespace {
+
+constexpr int kMaxH = 16384;
+constexpr int kBwdBlocks = 592;             // 4 per SM: fixed, so that the order of the partial sums does not follow the device
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+    f[4] = __uint_as_float(v.z << 16); f[5] = __uint_as_float(v.z & 0xffff0000u);
+    f[6] = __uint_as_float(v.w << 16); f[7] = __uint_as_float(v.w & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+}
+// VEC: whole 16-byte vectors (H % 8 == 0 and aligned rows); otherwise element by element, n of 8 valid.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int n) {
+    if (VEC) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint16_t* p, const uint4& v, int n) {
+    if (VEC) { *reinterpret_cast<uint4*>(p) = v; return; }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) p[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+// Sum over the block, the same value in every thread; `slot` is the copy of the partial sums this row uses.
+__device__ __forceinline__ float block_sum(float v, float* slot) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int nw = blockDim.x >> 5;
+    float t = 0.0f;
+    for (int w = 0; w < nw; ++w) t += slot[w];
+    return t;
+}
+
+struct NormParams {
+    const uint16_t* x;
+    const uint16_t* res;
+    const uint16_t* gain;
+    uint16_t* h;
+    uint16_t* normed;
+    float* rms;
+    uint8_t* out8;
+    long long ld_out8;
+    float* descale;
+    long long d_row, d_blk;
+    int rows, H;
+    float eps;
+    int vec8;
+};
+
+// x, res and h may be the same memory (every thread reads its own elements before it writes them): no __restrict__.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
+    __shared__ float s_sum[2][32];
+    const int nv = (p.H + 7) / 8;
+    int par = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
+        const long long base = row * p.H;
+        uint4 v[NV];
+        float acc = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int vi = threadIdx.x + blockDim.x * i;
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (vi < nv) v[i] = load8<VEC>(p.x + base + vi * 8, p.H - vi * 8);
+        }
+        if (p.res) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int vi = threadIdx.x + blockDim.x * i;
+                if (vi < nv) {
+                    float a[8], b[8];
+                    unpack8(v[i], a);
+                    unpack8(load8<VEC>(p.res + base + vi * 8, p.H - vi * 8), b);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) a[e] += b[e];
+                    v[i] = pack8(a);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[8];
+            unpack8(v[i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc = fmaf(f[e], f[e], acc);
+            const int vi = threadIdx.x + blockDim.x * i;
+            if (p.h && vi < nv) store8<VEC>(p.h + base + vi * 8, v[i], p.H - vi * 8);
+        }
+        const float total = block_sum(acc, s_sum[par]);
+        const float rms = sqrtf(__fdiv_rn(total, static_cast<float>(p.H)) + p.eps);
+        if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
+        const float inv = __fdiv_rn(1.0f, rms);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int vi = threadIdx.x + blockDim.x * i;
+            float f[8], g[8];
+            unpack8(v[i], f);
+            unpack8(vi < nv ? load8<VEC>(p.gain + vi * 8, p.H - vi * 8) : make_uint4(0u, 0u, 0u, 0u), g);
+            float a = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[e] = f[e] * inv * g[e];
+                a = fmaxf(a, fabsf(f[e]));
+            }
+            if (p.normed && vi < nv) store8<VEC>(p.normed + base + vi * 8, pack8(f), p.H - vi * 8);
+            if (p.out8) {                               // kernel-uniform: the half-warp holds one group of 128
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+                a = fmaxf(a, 1e-12f);
+                if (vi < nv) {
+                    const float s = __fdiv_rn(448.0f, a);
+                    const uint32_t q0 = cvt_fp8x4<false>(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
+                    const uint32_t q1 = cvt_fp8x4<false>(f[4] * s, f[5] * s, f[6] * s, f[7] * s);
+                    uint8_t* o = p.out8 + row * p.ld_out8 + vi * 8;
+                    if (VEC && p.vec8) {
+                        *reinterpret_cast<uint2*>(o) = make_uint2(q0, q1);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (vi * 8 + e < p.H) o[e] = static_cast<uint8_t>((e < 4 ? q0 >> (8 * e) : q1 >> (8 * (e - 4))) & 0xffu);
+                    }
+                    if ((threadIdx.x & 15) == 0) p.descale[row * p.d_row + (vi / 16) * p.d_blk] = __fdiv_rn(a, 448.0f);
+                }
+            }
+        }
+    }
+}
+
+struct NormGradParams {
+    const uint16_t* dy;
+    const uint16_t* h;
+    const uint16_t* gain;
+    const float* rms;
+    const uint16_t* dh;
+    uint16_t* dx;
+    float* partial;           // [gridDim.x, H] or null
+    int rows, H;
+};
+
+// dx may be the same memory as dy or dh.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(512) k_add_rmsnorm_grad(const NormGradParams p) {
+    __shared__ float s_sum[2][32];
+    const int nv = (p.H + 7) / 8;
+    float dg[NV][8];
+    uint4 gain[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int vi = threadIdx.x + blockDim.x * i;
+        gain[i] = vi < nv ? load8<VEC>(p.gain + vi * 8, p.H - vi * 8) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dg[i][e] = 0.0f;
+    }
+    int par = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
+        const long long base = row * p.H;
+        uint4 dy[NV], h[NV], dh[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int vi = threadIdx.x + blockDim.x * i;
+            dy[i] = h[i] = dh[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (vi < nv) {
+                dy[i] = load8<VEC>(p.dy + base + vi * 8, p.H - vi * 8);
+                h[i] = load8<VEC>(p.h + base + vi * 8, p.H - vi * 8);
+                if (p.dh) dh[i] = load8<VEC>(p.dh + base + vi * 8, p.H - vi * 8);
+            }
+        }
+        const float rms = p.rms[row];
+        const float inv = __fdiv_rn(1.0f, rms);
+        float acc = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float a[8], b[8], g[8];
+            unpack8(dy[i], a);
+            unpack8(h[i], b);
+            unpack8(gain[i], g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                acc = fmaf(a[e] * g[e], b[e] * inv, acc);
+                dg[i][e] = fmaf(a[e], b[e] * inv, dg[i][e]);
+            }
+        }
+        const float mean = __fdiv_rn(block_sum(acc, s_sum[par]), static_cast<float>(p.H));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int vi = threadIdx.x + blockDim.x * i;
+            float a[8], b[8], g[8], d[8];
+            unpack8(dy[i], a);
+            unpack8(h[i], b);
+            unpack8(gain[i], g);
+            unpack8(dh[i], d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(fmaf(-b[e] * inv, mean, a[e] * g[e]), inv, d[e]);
+            if (vi < nv) store8<VEC>(p.dx + base + vi * 8, pack8(d), p.H - vi * 8);
+        }
+    }
+    if (p.partial) {
+        float* o = p.partial + static_cast<long long>(blockIdx.x) * p.H;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int vi = threadIdx.x + blockDim.x * i;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (vi * 8 + e < p.H) o[vi * 8 + e] = dg[i][e];
+        }
+    }
+}
+
+// out[c] (+)= sum over the partial rows, in row order within each of the 32 warps of a block, then over the warps.
+__global__ void __launch_bounds__(1024) k_sum_partials(const float* __restrict__ partial, int n, int H, float* __restrict__ out, int accumulate) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
+    float t = 0.0f;
+    if (c < H)
+        for (int r = warp; r < n; r += 32) t += partial[static_cast<long long>(r) * H + c];
+    s[warp][lane] = t;
+    __syncthreads();
+    if (warp == 0 && c < H) {
+        float v = s[0][lane];
+#pragma unroll
+        for (int w = 1; w < 32; ++w) v += s[w][lane];
+        out[c] = accumulate ? out[c] + v : v;
+    }
+}
+
+// ------------------------------------------------------------------ host side
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+int threads_for(int nv, int per_thread) {
+    const int t = (nv + per_thread - 1) / per_thread;
+    return (t + 31) / 32 * 32;
+}
+
+template <int NV, bool VEC>
+int launch_forward(const NormParams& p, cudaStream_t st) {
+    const int t = threads_for((p.H + 7) / 8, NV);
+    int per_sm = 0;
+    CF_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_add_rmsnorm<NV, VEC>, t, 0));
+    long long grid = static_cast<long long>(sm_count()) * (per_sm < 1 ? 1 : per_sm);
+    if (grid > p.rows) grid = p.rows;
+    k_add_rmsnorm<NV, VEC><<<static_cast<unsigned>(grid), t, 0, st>>>(p);
+    CF_LAUNCH_CHECK("add_rmsnorm");
+    return CF_OK;
+}
+
+int grad_blocks(int rows, int H) {
+    const int t = threads_for((H + 7) / 8, 4);
+    int b = kBwdBlocks / 4 * (t <= 128 ? 4 : t <= 256 ? 2 : 1);
+    return b < rows ? b : rows;
+}
+
+}  // namespace
+}  // namespace cf
+
+using namespace cf;
+
+extern "C" {
+
+int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_null, const void* d_scale, void* d_h_or_null,
+                                     void* d_normed_or_null, float* d_rms_or_null, void* d_out8_or_null, int ld_out8, float* d_descale,
+                                     long long descale_ld_row, long long descale_ld_block, int rows, int H, float eps, void* stream) {
+    const char* fn = "cf_add_rmsnorm_quantize_block128";
+    CF_REQUIRE(rows >= 0 && H > 0, "%s: bad shape", fn);
+    if (H > kMaxH) { set_error("%s: rows of at most %d elements", fn, kMaxH); return CF_ERR_LIMIT; }
+    CF_REQUIRE(eps > 0.0f, "%s: eps must be positive", fn);
+    if (rows == 0) return CF_OK;
+    CF_REQUIRE((d_out8_or_null != nullptr) == (d_descale != nullptr), "%s: codes and descales go together", fn);
+    CF_REQUIRE(d_x && d_scale, "%s: null input", fn);
+    CF_REQUIRE(d_out8_or_null || d_normed_or_null, "%s: no output", fn);
+    CF_REQUIRE(d_h_or_null || !d_residual_or_null, "%s: the sum with a residual needs a buffer", fn);
+    CF_REQUIRE(!d_out8_or_null || ld_out8 >= H, "%s: output pitch smaller than a row", fn);
+    CF_REQUIRE(aligned(d_x, 2) && aligned(d_residual_or_null, 2) && aligned(d_scale, 2) && aligned(d_h_or_null, 2) &&
+               aligned(d_normed_or_null, 2) && aligned(d_rms_or_null, 4) && aligned(d_descale, 4), "%s: misaligned pointer", fn);
+    const int rc = require_sm100();
+    if (rc != CF_OK) return rc;
+    NormParams p = {};
+    p.x = static_cast<const uint16_t*>(d_x); p.res = static_cast<const uint16_t*>(d_residual_or_null);
+    p.gain = static_cast<const uint16_t*>(d_scale);
+    p.h = static_cast<uint16_t*>(d_h_or_null); p.normed = static_cast<uint16_t*>(d_normed_or_null);
+    p.rms = d_rms_or_null; p.out8 = static_cast<uint8_t*>(d_out8_or_null); p.ld_out8 = ld_out8;
+    p.descale = d_descale; p.d_row = descale_ld_row; p.d_blk = descale_ld_block;
+    p.rows = rows; p.H = H; p.eps = eps;
+    p.vec8 = aligned(d_out8_or_null, 8) && ld_out8 % 8 == 0;
+    const bool vec = H % 8 == 0 && aligned(d_x, 16) && aligned(d_residual_or_null, 16) && aligned(d_scale, 16) &&
+                     aligned(d_h_or_null, 16) && aligned(d_normed_or_null, 16);
+    cudaStream_t st = as_stream(stream);
+    if (!vec) return launch_forward<4, false>(p, st);
+    return launch_forward<4, true>(p, st);
+}
+
+size_t cf_add_rmsnorm_backward_scratch_floats(int rows, int H) {
+    if (rows <= 0 || H <= 0 || H > kMaxH) return 0;
+    return static_cast<size_t>(grad_blocks(rows, H)) * H;
+}
+
+int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_scale, const float* d_rms, const void* d_dh_or_null, void* d_dx,
+                            float* d_dscale_or_null, int accumulate_dscale, float* d_scratch, size_t scratch_floats, int rows, int H,
+                            void* stream) {
+    const char* fn = "cf_add_rmsnorm_backward";
+    CF_REQUIRE(rows >= 0 && H > 0, "%s: bad shape", fn);
+    if (H > kMaxH) { set_error("%s: rows of at most %d elements", fn, kMaxH); return CF_ERR_LIMIT; }
+    CF_REQUIRE(aligned(d_dscale_or_null, 4) && aligned(d_rms, 4) && aligned(d_scratch, 4), "%s: misaligned pointer", fn);
+    cudaStream_t st = as_stream(stream);
+    if (rows == 0) {                                    // a sum over no rows
+        if (d_dscale_or_null && !accumulate_dscale) CF_CUDA(cudaMemsetAsync(d_dscale_or_null, 0, sizeof(float) * H, st));
+        return CF_OK;
+    }
+    CF_REQUIRE(d_dy && d_h && d_scale && d_rms && d_dx, "%s: null pointer", fn);
+    CF_REQUIRE(aligned(d_dy, 2) && aligned(d_h, 2) && aligned(d_scale, 2) && aligned(d_dh_or_null, 2) && aligned(d_dx, 2), "%s: misaligned pointer", fn);
+    const size_t need = cf_add_rmsnorm_backward_scratch_floats(rows, H);
+    if (d_dscale_or_null && (!d_scratch || scratch_floats < need)) {
+        set_error("%s: %zu floats of scratch needed", fn, need);
+        return CF_ERR_LIMIT;
+    }
+    const int rc = require_sm100();
+    if (rc != CF_OK) return rc;
+    NormGradParams p = {};
+    p.dy = static_cast<const uint16_t*>(d_dy); p.h = static_cast<const uint16_t*>(d_h); p.gain = static_cast<const uint16_t*>(d_scale);
+    p.rms = d_rms; p.dh = static_cast<const uint16_t*>(d_dh_or_null); p.dx = static_cast<uint16_t*>(d_dx);
+    p.partial = d_dscale_or_null ? d_scratch : nullptr;
+    p.rows = rows; p.H = H;
+    const bool vec = H % 8 == 0 && aligned(d_dy, 16) && aligned(d_h, 16) && aligned(d_scale, 16) && aligned(d_dh_or_null, 16) && aligned(d_dx, 16);
+    const int t = threads_for((H + 7) / 8, 4), blocks = grad_blocks(rows, H);
+    if (vec) k_add_rmsnorm_grad<4, true><<<blocks, t, 0, st>>>(p);
+    else k_add_rmsnorm_grad<4, false><<<blocks, t, 0, st>>>(p);
+    CF_LAUNCH_CHECK("add_rmsnorm_grad");
+    if (d_dscale_or_null) {
+        k_sum_partials<<<(H + 31) / 32, 1024, 0, st>>>(d_scratch, blocks, H, d_dscale_or_null, accumulate_dscale);
+        CF_LAUNCH_CHECK("sum_partials");
+    }
+    return CF_OK;
+}
+
+}  // extern "C"

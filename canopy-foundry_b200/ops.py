@@ -26,6 +26,9 @@ __all__ = [
     "moe_topk_route_f32", "moe_build_expert_row_lists", "moe_expert_offsets_from_counts",
     "moe_gather_rows_u8", "moe_gather_rows_bf16", "moe_scatter_accumulate_rows_bf16",
     "moe_scale_accumulate_bf16", "moe_gather_all_u8", "moe_combine_all_bf16", "moe_combine_sorted_bf16", "moe_expand_route_replicas", "moe_route_dispatch_lists", "moe_route_dispatch_scratch_ints", "moe_ep_plan", "gemm_fp8_nt_grouped_return", "moe_send_row_runs", "peer_barrier", "peer_share_i32", "ROW_RUN_BYTES",
+    "block128_row_descale", "fp8_quantize_block128", "swiglu_quantize_block128", "swiglu_backward_quantize_block128", "fp8_quantize_block128x128",
+    "add_rmsnorm_quantize_block128", "add_rmsnorm_backward", "add_rmsnorm_backward_scratch_floats",
+    "gemm_fp8_block128_nt", "gemm_fp8_block128_nt_grouped", "gemm_fp8_block128_nn", "gemm_fp8_block128_dw",
     "moe_grouped_expert_forward_fp8", "launch_count", "swiglu_mlp_fp8_rowwise", "MoeSwigluFp8", "FfnSwigluFp8",
 ]
 
@@ -566,6 +569,194 @@ def moe_grouped_expert_forward_fp8(ctx, hidden, fcin_descale, fcin_is_e5m2, rout
                                                  _p(route_weights), _p(counts), _p(offsets), _p(row_indices),
                                                  _p(fc_in_w), _p(fc_in_descale), _p(fc_out_w), _p(fc_out_descale),
                                                  _p(mixed), rows, H, Ie, num_experts, total_selected_rows, _s()))
+
+
+# ---------------------------------------------------------------- block-scaled FP8 (one scale per 128 values)
+BLOCK = 128
+
+
+def _need(ok, what):
+    """A call whose tensors do not fit together is refused before any pointer reaches the library."""
+    if not ok:
+        raise CanopyError(_capi.CF_ERR_INVALID_ARG, what)
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def _mat(t, dtypes, shape, what):
+    """[rows, cols] tensor with unit stride along the columns; its row pitch."""
+    _need(t.dtype in dtypes, f"{what}: type {t.dtype}")
+    _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)), f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{what}: columns must be contiguous")
+    if t.shape[0] <= 1:
+        return -(-t.shape[1] // 16) * 16               # the pitch of a single row addresses no memory
+    _need(t.stride(0) >= t.shape[1], f"{what}: rows must not overlap")
+    return t.stride(0)
+
+
+def _scales(t, shape, what):
+    _need(t.dtype == torch.float32 and tuple(t.shape) == tuple(shape), f"{what}: float32 {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
+    return t.stride(0), t.stride(1)
+
+
+_BF16, _CODES, _OUT = (torch.bfloat16,), (torch.uint8,), (torch.bfloat16, torch.float32)
+
+
+def block128_row_descale(rows, cols, device="cuda"):
+    """Descales of row groups, [rows, ceil(cols / 128)], the rows next to each other in memory (what the GEMM reads best)."""
+    return torch.empty((_blocks(cols), rows), dtype=torch.float32, device=device).t()
+
+
+def _group_outputs(rows, cols, row8, row_descale, col8, col_descale):
+    _need((row8 is None) == (row_descale is None) and (col8 is None) == (col_descale is None), "codes and descales go together")
+    _need(row8 is not None or col8 is not None, "no output")
+    r = (None, 0, None, 0, 0) if row8 is None else (_p(row8), _mat(row8, _CODES, (rows, cols), "row8"), _p(row_descale),
+                                                    *_scales(row_descale, (rows, _blocks(cols)), "row_descale"))
+    c = (None, 0, None, 0, 0) if col8 is None else (_p(col8), _mat(col8, _CODES, (rows, cols), "col8"), _p(col_descale),
+                                                    *_scales(col_descale, (_blocks(rows), cols), "col_descale"))
+    return r + c
+
+
+def fp8_quantize_block128(x, row8=None, row_descale=None, col8=None, col_descale=None, is_e5m2=False):
+    """Codes of a bf16 matrix with one scale per 128 values of a row (row8, row_descale [rows, ceil(cols/128)]) and / or per
+    128 values of a column (col8, col_descale [ceil(rows/128), cols]), from one read."""
+    rows, cols = x.shape
+    check(_L().cf_fp8_quantize_block128(_p(x), _mat(x, _BF16, None, "x"), rows, cols, int(is_e5m2),
+                                        *_group_outputs(rows, cols, row8, row_descale, col8, col_descale), _s()))
+
+
+def swiglu_quantize_block128(gate, up, row8=None, row_descale=None, col8=None, col_descale=None):
+    """fp8_quantize_block128 of silu(gate) * up (E4M3, no bf16 rounding in between); gate and up share a row pitch."""
+    rows, cols = gate.shape
+    ld = _mat(gate, _BF16, None, "gate")
+    _need(_mat(up, _BF16, (rows, cols), "up") == ld, "gate and up must have the same row pitch")
+    check(_L().cf_swiglu_quantize_block128(_p(gate), _p(up), ld, rows, cols,
+                                           *_group_outputs(rows, cols, row8, row_descale, col8, col_descale), _s()))
+
+
+def swiglu_backward_quantize_block128(gate, up, dh, row8=None, row_descale=None, col8=None, col_descale=None, is_e5m2=False):
+    """Codes of the gradient of silu(gate) * up: [rows, 2 cols], d gate first, d up behind it; cols a multiple of 128."""
+    rows, cols = gate.shape
+    ld = _mat(gate, _BF16, None, "gate")
+    _need(_mat(up, _BF16, (rows, cols), "up") == ld, "gate and up must have the same row pitch")
+    check(_L().cf_swiglu_backward_quantize_block128(_p(gate), _p(up), ld, _p(dh), _mat(dh, _BF16, (rows, cols), "dh"), rows, cols,
+                                                    int(is_e5m2), *_group_outputs(rows, 2 * cols, row8, row_descale, col8, col_descale),
+                                                    _s()))
+
+
+def fp8_quantize_block128x128(w, w8, descale):
+    """E4M3 codes of a weight [rows, cols], or of a stack [n, rows, cols], with one scale per 128x128 block
+    (descale [..., ceil(rows/128), ceil(cols/128)])."""
+    _need(w.dim() in (2, 3) and w8.shape == w.shape and descale.dim() == w.dim(), "weight, codes and descales: shapes differ")
+    n = w.shape[0] if w.dim() == 3 else 1
+    rows, cols = w.shape[-2:]
+    if n == 0 or rows == 0 or cols == 0:
+        return
+    stacked = w.dim() == 3
+    _need(descale.dtype == torch.float32 and tuple(descale.shape) == (*w.shape[:-2], _blocks(rows), _blocks(cols)) and
+          (descale.stride(-1) == 1 or descale.shape[-1] == 1), "descale: float32 with contiguous rows of blocks expected")
+    w0, q0, d0 = (w[0], w8[0], descale[0]) if stacked else (w, w8, descale)
+    ld_d = d0.stride(0) if d0.shape[0] > 1 else max(d0.stride(0), d0.shape[1])
+    check(_L().cf_fp8_quantize_block128x128(_p(w), _mat(w0, _BF16, None, "w"), w.stride(0) if stacked else 0, n, rows, cols, _p(w8),
+                                            _mat(q0, _CODES, None, "w8"), w8.stride(0) if stacked else 0, _p(descale), ld_d,
+                                            descale.stride(0) if stacked else 0, _s()))
+
+
+def add_rmsnorm_quantize_block128(x, residual, scale, h, rms=None, normed=None, out8=None, descale=None, eps=1e-6):
+    """h = bf16(x + residual), RMS norm of h with gain `scale`, codes and row-group descales of the normalised row (and / or
+    its bf16 copy `normed`), in one pass. residual may be None (then h may be, too); h may be x or residual itself."""
+    rows, H = x.shape
+    for t, what in ((x, "x"), (residual, "residual"), (h, "h"), (normed, "normed")):
+        _need(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, H) and t.is_contiguous()),
+              f"{what}: contiguous bf16 [{rows}, {H}] expected")
+    _need(scale.dtype == torch.bfloat16 and scale.numel() == H and scale.is_contiguous(), "scale: contiguous bf16 [H] expected")
+    _need(rms is None or (rms.dtype == torch.float32 and rms.numel() == rows and rms.is_contiguous()), "rms: contiguous float32 [rows] expected")
+    _need((out8 is None) == (descale is None), "codes and descales go together")
+    ld8, dr, db = (0, 0, 0) if out8 is None else (_mat(out8, _CODES, (rows, H), "out8"), *_scales(descale, (rows, _blocks(H)), "descale"))
+    check(_L().cf_add_rmsnorm_quantize_block128(_p(x), _p(residual), _p(scale), _p(h), _p(normed), _p(rms), _p(out8), ld8, _p(descale),
+                                                dr, db, rows, H, eps, _s()))
+
+
+def add_rmsnorm_backward_scratch_floats(rows, H):
+    return int(_L().cf_add_rmsnorm_backward_scratch_floats(rows, H))
+
+
+def add_rmsnorm_backward(dy, h, scale, rms, dh, dx, dscale=None, scratch=None, accumulate_dscale=False):
+    """Gradient of the residual addition + RMS norm: dx (of x and of the residual alike) from dy and the gradient dh of the
+    residual stream (or None); dscale float32 [H], stored or added to, or None. dx may be dy or dh itself."""
+    rows, H = h.shape
+    for t, what in ((dy, "dy"), (h, "h"), (dh, "dh"), (dx, "dx")):
+        _need(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, H) and t.is_contiguous()),
+              f"{what}: contiguous bf16 [{rows}, {H}] expected")
+    _need(scale.dtype == torch.bfloat16 and scale.numel() == H and scale.is_contiguous(), "scale: contiguous bf16 [H] expected")
+    _need(rms.dtype == torch.float32 and rms.numel() == rows and rms.is_contiguous(), "rms: contiguous float32 [rows] expected")
+    _need(dscale is None or (dscale.dtype == torch.float32 and dscale.numel() == H and dscale.is_contiguous()), "dscale: contiguous float32 [H] expected")
+    _need(scratch is None or (scratch.dtype == torch.float32 and scratch.is_contiguous()), "scratch: contiguous float32 expected")
+    check(_L().cf_add_rmsnorm_backward(_p(dy), _p(h), _p(scale), _p(rms), _p(dh), _p(dx), _p(dscale), int(accumulate_dscale), _p(scratch),
+                                       0 if scratch is None else scratch.numel(), rows, H, _s()))
+
+
+def _out_args(out, M, N):
+    return _p(out), _mat(out, _OUT, (M, N), "out"), int(out.dtype == torch.float32)
+
+
+def gemm_fp8_block128_nt(ctx, A8, a_descale, B8, b_descale, out, a_is_e5m2=False, accumulate=False):
+    """out[M,N] (bf16 or float32) = A8[M,K] . B8[N,K]^T with a_descale [M, ceil(K/128)] and b_descale [ceil(N/128), ceil(K/128)]
+    (128x128 blocks, weights) or [N, ceil(K/128)] (row groups; taken for blocks where the two shapes are the same, N = 1)."""
+    (M, K), N = A8.shape, B8.shape[0]
+    per = BLOCK if b_descale.shape[0] == _blocks(N) else 1
+    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8, _CODES, (N, K), "B8")
+    sa = _scales(a_descale, (M, _blocks(K)), "a_descale")
+    sb = _scales(b_descale, (_blocks(N) if per == BLOCK else N, _blocks(K)), "b_descale")
+    c, ldc, f32 = _out_args(out, M, N)
+    check(_L().cf_gemm_fp8_block128_nt(ctx.handle, M, N, K, _p(A8), lda, int(a_is_e5m2), _p(a_descale), *sa, _p(B8), ldb,
+                                       _p(b_descale), *sb, per, c, ldc, f32, int(accumulate), _s()))
+
+
+def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_descale, out, a_is_e5m2=False):
+    """Rows [offsets[e], +counts[e]) of the compact A8 times expert e of the stacked B8 [E, N, K] (b_descale
+    [E, ceil(N/128), ceil(K/128)]) into the same rows of the bf16 out; the other rows are left as they are."""
+    (T, K), (E, N, _) = A8.shape, B8.shape
+    _need(counts.dtype == torch.int32 and offsets.dtype == torch.int32 and counts.numel() == E and offsets.numel() == E and
+          counts.is_contiguous() and offsets.is_contiguous(), "counts, offsets: contiguous int32 [E] expected")
+    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8[0], _CODES, (N, K), "B8")
+    if N == 1 and E > 1:
+        ldb = B8.stride(0)
+    _need(E == 1 or B8.stride(0) == N * ldb, "B8: the experts must lie behind one another")
+    sa = _scales(a_descale, (T, _blocks(K)), "a_descale")
+    _need(b_descale.dtype == torch.float32 and tuple(b_descale.shape) == (E, _blocks(N), _blocks(K)) and
+          (b_descale.stride(2) == 1 or b_descale.shape[2] == 1), "b_descale: float32 [E, ceil(N/128), ceil(K/128)] expected")
+    _need(out.dtype == torch.bfloat16, "out: bf16 expected")
+    c, ldc, _ = _out_args(out, T, N)
+    check(_L().cf_gemm_fp8_block128_nt_grouped(ctx.handle, E, T, N, K, _p(counts), _p(offsets), _p(A8), lda, int(a_is_e5m2),
+                                               _p(a_descale), *sa, _p(B8), ldb, _p(b_descale), b_descale.stride(1),
+                                               b_descale.stride(0), c, ldc, _s()))
+
+
+def gemm_fp8_block128_nn(ctx, A8, a_descale, B8_kn, b_descale, out, a_is_e5m2=False, accumulate=False):
+    """Data gradient: out[M,N] = A8[M,K] . B8[K,N], the weight read from its forward cache ([out, in] = [K, N]) and block descales
+    [ceil(K/128), ceil(N/128)] as they lie; A8 (the gradient) with row groups along K."""
+    (M, K), N = A8.shape, B8_kn.shape[1]
+    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8_kn, _CODES, (K, N), "B8_kn")
+    sa = _scales(a_descale, (M, _blocks(K)), "a_descale")
+    sb = _scales(b_descale, (_blocks(K), _blocks(N)), "b_descale")
+    _need(sb[1] == 1 or _blocks(N) == 1, "b_descale: rows of blocks must be contiguous")
+    c, ldc, f32 = _out_args(out, M, N)
+    check(_L().cf_gemm_fp8_block128_nn(ctx.handle, M, N, K, _p(A8), lda, int(a_is_e5m2), _p(a_descale), *sa, _p(B8_kn), ldb,
+                                       _p(b_descale), sb[0], c, ldc, f32, int(accumulate), _s()))
+
+
+def gemm_fp8_block128_dw(ctx, X8, x_descale, dY8, dy_descale, dW, x_is_e5m2=False, dy_is_e5m2=False, accumulate=False):
+    """Weight gradient: dW[M,N] (float32 or bf16) = X8[T,M]^T . dY8[T,N] over T tokens, both with column groups of 128 tokens
+    (descales [ceil(T/128), M] and [ceil(T/128), N])."""
+    (T, M), N = X8.shape, dY8.shape[1]
+    ldx, ldy = _mat(X8, _CODES, None, "X8"), _mat(dY8, _CODES, (T, N), "dY8")
+    sx, sy = _scales(x_descale, (_blocks(T), M), "x_descale"), _scales(dy_descale, (_blocks(T), N), "dy_descale")
+    c, ldc, f32 = _out_args(dW, M, N)
+    check(_L().cf_gemm_fp8_block128_dw(ctx.handle, M, N, T, _p(X8), ldx, int(x_is_e5m2), _p(x_descale), *sx, _p(dY8), ldy,
+                                       int(dy_is_e5m2), _p(dy_descale), *sy, c, ldc, f32, int(accumulate), _s()))
 
 
 # ---------------------------------------------------------------- composites: SwiGLU MLP (per-token scales) and MoE SwiGLU experts

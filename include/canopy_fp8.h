@@ -449,6 +449,100 @@ int cf_swiglu_quantize_rowwise_e4m3(const void* d_gate, const void* d_up, int ld
 int cf_swiglu_quantize_e4m3_record(const void* d_gate, const void* d_up, int ld_in, void* d_out, int ld_out,
                                    const float* d_scale, float* d_amax, int rows, int cols, void* stream);
 
+/* ------------------------------------------------------------------ block-scaled FP8 (one scale per 128 values)
+ *
+ * No counterpart in the reference, which scales per tensor; the formulas generalise kernels/fp8.cu:34-49 to groups of 128:
+ *   a = max(max|v| over the group, 1e-12), descale = a / FMAX, code = fp8(v * (FMAX / a)),  FMAX = 448 (E4M3) or 57344 (E5M2)
+ * Groups: 1x128 along a row (operands contracted along the row), 128x1 down a column (operands of the weight gradient,
+ * contracted over tokens), 128x128 blocks (weights). The last group of a row or column may be shorter. Descales are fp32 and
+ * addressed by strides in elements, so they may lie [rows, groups], [groups, rows] (what coalesces best in the GEMM) or
+ * inside larger buffers: row descale of (r, b) at d[r * ld_row + b * ld_block], column descale of (b, c) at
+ * d[b * ld_block + c * ld_col]. NaN is ignored by the amax and coded as NaN; a group that holds an infinity gets descale +Inf
+ * and contributes NaN. Any number of rows and columns and any pitch; 16-byte aligned inputs with pitches that are multiples
+ * of 8 elements, and 8-byte aligned codes with pitches that are multiples of 8, take vector accesses. The GEMMs need
+ * 16-byte aligned codes with pitches that are multiples of 16 (the columns behind a row's end are not read). */
+
+/* bf16 [rows, cols] (pitch ld_x) -> codes with row groups and / or codes with column groups, from one read. A pair of
+ * codes and descales is left out by passing NULL for both. */
+int cf_fp8_quantize_block128(const void* d_x, int ld_x, int rows, int cols, int is_e5m2, void* d_row8_or_null, int ld_row8,
+                             float* d_row_descale, long long row_descale_ld_row, long long row_descale_ld_block, void* d_col8_or_null,
+                             int ld_col8, float* d_col_descale, long long col_descale_ld_block, long long col_descale_ld_col, void* stream);
+/* The same on silu(gate) * up (kernels/activations.cu:28-40), E4M3. The product is NOT rounded to bf16 on its way: one
+ * rounding, to the code. gate and up are [rows, cols] views with row pitch ld_in. */
+int cf_swiglu_quantize_block128(const void* d_gate, const void* d_up, int ld_in, int rows, int cols, void* d_row8_or_null, int ld_row8,
+                                float* d_row_descale, long long row_descale_ld_row, long long row_descale_ld_block,
+                                void* d_col8_or_null, int ld_col8, float* d_col_descale, long long col_descale_ld_block,
+                                long long col_descale_ld_col, void* stream);
+/* The same on the gradient of silu(gate) * up for an arriving gradient dh [rows, cols] (bf16, pitch ld_dh):
+ *   d gate = dh up sig(gate) (1 + gate (1 - sig(gate))),  d up = dh silu(gate)
+ * The outputs are [rows, 2 cols], d gate in columns [0, cols) and d up behind it, like the product of a stacked gate/up
+ * weight. cols must be a multiple of 128. */
+int cf_swiglu_backward_quantize_block128(const void* d_gate, const void* d_up, int ld_in, const void* d_dh, int ld_dh, int rows, int cols,
+                                         int is_e5m2, void* d_row8_or_null, int ld_row8, float* d_row_descale,
+                                         long long row_descale_ld_row, long long row_descale_ld_block, void* d_col8_or_null,
+                                         int ld_col8, float* d_col_descale, long long col_descale_ld_block, long long col_descale_ld_col,
+                                         void* stream);
+/* Weights: num_weights matrices [rows, cols] (bf16, row pitch ld_w, w_stride elements apart) -> E4M3 codes (row pitch ld_out,
+ * out_stride bytes apart) with one descale per 128x128 block, [ceil(rows/128), ceil(cols/128)] with row pitch descale_ld_row,
+ * descale_stride apart. Blocks restart in every matrix. The strides are ignored when num_weights is 1. */
+int cf_fp8_quantize_block128x128(const void* d_w, int ld_w, long long w_stride, int num_weights, int rows, int cols, void* d_out8,
+                                 int ld_out, long long out_stride, float* d_descale, long long descale_ld_row, long long descale_stride,
+                                 void* stream);
+
+/* Residual addition + RMS norm (kernels/rmsnorm.cu:13-54 computes the norm alone) + row-group quantisation in one pass:
+ *   h = bf16(x + residual); rms = sqrt(mean(h^2) + eps); y = (h / rms) * scale; codes and descales of y
+ * x, residual, h, normed: bf16 [rows, H] contiguous, scale bf16 [H], rms float[rows]. Without a residual h = x and d_h may be
+ * NULL. h may be the same memory as x or residual. y goes to the codes from fp32; d_normed_or_null receives bf16(y) (the
+ * codes may then be left out). eps > 0. At most 16384 elements a row. */
+int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_null, const void* d_scale, void* d_h_or_null,
+                                     void* d_normed_or_null, float* d_rms_or_null, void* d_out8_or_null, int ld_out8, float* d_descale,
+                                     long long descale_ld_row, long long descale_ld_block, int rows, int H, float eps, void* stream);
+/* Its gradient, for the arriving gradients dy of y and dh (or NULL) of h:
+ *   u = dy * scale;  dx = (u - (h / rms) * mean(u * h / rms)) / rms + dh   (the gradient of x and of residual alike)
+ *   dscale[c] (+)= sum over rows of dy * h / rms                         (fp32; NULL: not wanted, no scratch needed)
+ * dx may be the same memory as dy or dh. d_scratch: cf_add_rmsnorm_backward_scratch_floats(rows, H) floats owned by the
+ * caller, contents irrelevant (CF_ERR_LIMIT if too small); two calls that overlap on the GPU need scratch of their own.
+ * The sums are taken in an order that depends on rows and H alone. */
+size_t cf_add_rmsnorm_backward_scratch_floats(int rows, int H);
+int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_scale, const float* d_rms, const void* d_dh_or_null, void* d_dx,
+                            float* d_dscale_or_null, int accumulate_dscale, float* d_scratch, size_t scratch_floats, int rows, int H,
+                            void* stream);
+
+/* C[M,N] = sum over blocks b of 128 along K of da[m,b] * db[n,b] * sum_{k in b} A8[m,k] * B8[n,k]: block sums on the tensor
+ * cores, scaled and added up in fp32, one rounding to the output type.
+ * A8 [M, K] E4M3 or E5M2, row pitch lda; B8 [N, K] E4M3, row pitch ldb; both 16-byte aligned with pitches that are multiples
+ * of 16 (CF_ERR_UNSUPPORTED otherwise), K any number. b_rows_per_scale: 128 (weights: db of row n at
+ * d[(n / 128) * ld_row + b * ld_block]) or 1 (row groups). C: bf16 or (out_fp32) float, pitch ldc, stored or (accumulate)
+ * added to. No float atomics: results do not depend on timing. Up to 128 rows of A take a form that reads every weight
+ * once, with the contraction split over a cluster. */
+int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                            long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb, const float* d_b_descale,
+                            long long b_descale_ld_row, long long b_descale_ld_block, int b_rows_per_scale, void* d_C, int ldc,
+                            int out_fp32, int accumulate, void* stream);
+/* The same for ragged expert groups with a device-side schedule: compact rows [d_offsets[e], +d_counts[e]) times block e of
+ * the stacked weights [num_experts * N, K] (row pitch ldb), whose descales lie [ceil(N/128), ceil(K/128)] with row pitch
+ * b_descale_ld_row and unit block stride, b_descale_stride apart per expert. All compact buffers have max_total_rows rows;
+ * rows outside of them are never touched (a group is cut to them, one that starts outside is skipped), rows of no group are
+ * left as they are. bf16 output, forward only. */
+int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_rows, int N, int K, const int* d_counts,
+                                    const int* d_offsets, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                                    long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb,
+                                    const float* d_b_descale, long long b_descale_ld_row, long long b_descale_stride, void* d_C, int ldc,
+                                    void* stream);
+/* Data gradient: C[M,N] = A8[M,K] . B8[K,N] with the weight read from the forward cache as it lies ([out, in] = [K, N], row
+ * pitch ldb) and its 128x128 descales [ceil(K/128), ceil(N/128)] (row pitch b_descale_ld_row, unit stride along N). A8 has
+ * row groups along K. */
+int cf_gemm_fp8_block128_nn(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
+                            long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B_kn, int ldb,
+                            const float* d_b_descale, long long b_descale_ld_row, void* d_C, int ldc, int out_fp32, int accumulate,
+                            void* stream);
+/* Weight gradient: dW[M,N] (+)= X8[K,M]^T . dY8[K,N] over K tokens, both operands as they lie with column groups of 128
+ * tokens (descales of block b and column c at d[b * ld_block + c * ld_col]). */
+int cf_gemm_fp8_block128_dw(cf_ctx* ctx, int M, int N, int K, const void* d_X, int ldx, int x_is_e5m2, const float* d_x_descale,
+                            long long x_descale_ld_block, long long x_descale_ld_col, const void* d_dY, int ldy, int dy_is_e5m2,
+                            const float* d_dy_descale, long long dy_descale_ld_block, long long dy_descale_ld_col, void* d_dW, int ldc,
+                            int out_fp32, int accumulate, void* stream);
+
 /* ------------------------------------------------------------------ MoE routing, permute, combine */
 
 /* kernels/moe.cu:410-422, kernels.hpp:313-317: softmax in place, hard top-k (lowest index wins ties),

@@ -1,0 +1,510 @@
+"""Block-scaled FP8 operators (one scale per 128 values) against their definitions in 64 bits.
+
+Tolerances count roundings: a rounding to a type is off by at most eps / 2 of the value (bf16 2^-8, E4M3 2^-4, E5M2 2^-3, and
+half the smallest subnormal of the FP8 types below their normal range), and every fp32 operation by 2^-24 of its result."""
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import package
+
+pytestmark = pytest.mark.gpu
+
+G = 128
+FMAX = {False: 448.0, True: 57344.0}
+TYPE = {False: torch.float8_e4m3fn, True: torch.float8_e5m2}
+HALF = {False: 2.0 ** -4, True: 2.0 ** -3}          # half a step, relative
+TINY = {False: 2.0 ** -10, True: 2.0 ** -17}        # half the smallest subnormal
+U = 2.0 ** -24                                       # fp32 rounding
+
+
+@pytest.fixture(scope="module")
+def cfb():
+    return package()
+
+
+@pytest.fixture(scope="module")
+def ctx(cfb):
+    c = cfb.Fp8Ctx()
+    yield c
+    c.poll_status()
+    c.close()
+
+
+def cdiv(a, b):
+    return -(-a // b)
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(shape, seed, std=1.0):
+    return (torch.randn(shape, generator=gen(seed), device="cuda") * std).to(torch.bfloat16)
+
+
+def pitched(rows, cols, dtype, pad, offset=0, fill=0x5a):
+    """A [rows, cols] view with `pad` extra elements per row, `offset` elements into its buffer, and the buffer's bytes."""
+    size = torch.empty((), dtype=dtype).element_size()
+    raw = torch.full(((rows * (cols + pad) + offset + 64) * size,), fill, dtype=torch.uint8, device="cuda")
+    flat = raw.view(dtype)[offset:]
+    return flat[: rows * (cols + pad)].view(rows, cols + pad)[:, :cols], raw
+
+
+def decode(codes, e5m2):
+    return codes.contiguous().view(TYPE[e5m2]).double()
+
+
+def groups64(v, dim):
+    """max |v| of groups of 128 along dim, floored, in v's shape (spread over the group) and per group."""
+    n = v.shape[dim]
+    per = torch.stack([p.abs().amax(dim) for p in torch.split(v, G, dim)], dim).clamp(min=1e-12)
+    return per.repeat_interleave(G, dim).narrow(dim, 0, n), per
+
+
+def check_groups(codes, descale, v, dim, e5m2, slack):
+    """codes * descale is v up to one rounding to the type, descale is amax / FMAX; slack: relative fp32 error of v itself."""
+    a, per = groups64(v, dim)
+    assert (descale.double() - per / FMAX[e5m2]).abs().le((slack + 2 * U) * per / FMAX[e5m2]).all()
+    want = v / a * FMAX[e5m2]
+    err = (decode(codes, e5m2) - want).abs()
+    # v's own error and three fp32 operations (the scale's division, the product, the amax) move the value before it is rounded
+    bound = torch.maximum(want.abs() * HALF[e5m2], torch.full_like(want, TINY[e5m2])) * (1 + 2.0 ** -10) + want.abs() * (slack + 4 * U)
+    assert err.le(bound).all(), float((err - bound).max())
+
+
+def plain_codes(x, dim, e5m2):
+    """The same fp32 operations in torch: bit-exact codes and descales of a bf16 matrix. (Quotients are taken in 64 bits and
+    rounded, which is the IEEE fp32 quotient; torch's own division by or of a scalar goes through a rounded reciprocal.)"""
+    a, per = groups64(x.double(), dim)
+    a, per = a.float().double(), per.float().double()
+    q = (x.float() * (FMAX[e5m2] / a).float()).clamp(-FMAX[e5m2], FMAX[e5m2]).to(TYPE[e5m2])
+    return q.view(torch.uint8), (per / FMAX[e5m2]).float()
+
+
+# ---------------------------------------------------------------- quantiser
+SHAPES = [(1, 1), (1, 4096), (3, 127), (128, 128), (129, 257), (130, 136), (300, 1000), (1027, 513), (16, 8), (2048, 1024)]
+
+
+@pytest.mark.parametrize("e5m2", [False, True])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantise_rows_and_columns_bit_exact(cfb, rows, cols, e5m2):
+    x = normal((rows, cols), rows * 7 + cols)
+    if cols > 4:
+        x[0, 3] = 30.0
+    x[rows // 2] = 0.0                                   # a row of zeros: the floor of the amax
+    for which in ("row", "col", "both"):
+        row8 = torch.empty((rows, cols), dtype=torch.uint8, device="cuda") if which != "col" else None
+        rd = torch.empty((rows, cdiv(cols, G)), device="cuda") if which != "col" else None
+        col8 = torch.empty((rows, cols), dtype=torch.uint8, device="cuda") if which != "row" else None
+        cd = torch.empty((cdiv(rows, G), cols), device="cuda") if which != "row" else None
+        cfb.fp8_quantize_block128(x, row8, rd, col8, cd, is_e5m2=e5m2)
+        if which != "col":
+            q, d = plain_codes(x, 1, e5m2)
+            assert torch.equal(row8, q) and torch.equal(rd, d), which
+        if which != "row":
+            q, d = plain_codes(x, 0, e5m2)
+            assert torch.equal(col8, q) and torch.equal(cd, d), which
+        if which == "both":
+            check_groups(row8, rd, x.double(), 1, e5m2, 0.0)
+            check_groups(col8, cd, x.double(), 0, e5m2, 0.0)
+
+
+@pytest.mark.parametrize("pad,offset", [(0, 1), (1, 0), (8, 8), (3, 5)])
+def test_quantise_pitches_and_alignments_leave_the_rest(cfb, pad, offset):
+    rows, cols = 141, 261
+    x, _ = pitched(rows, cols, torch.bfloat16, pad, offset)
+    x.copy_(normal((rows, cols), 3))
+    row8, raw_r = pitched(rows, cols, torch.uint8, pad, offset)
+    col8, raw_c = pitched(rows, cols, torch.uint8, pad, offset)
+    rd = cfb.block128_row_descale(rows, cols)            # [groups, rows] in memory
+    cd = torch.full((cols, cdiv(rows, G)), -1.0, device="cuda").t()
+    cfb.fp8_quantize_block128(x, row8, rd, col8, cd)
+    q, d = plain_codes(x, 1, False)
+    assert torch.equal(row8, q) and torch.equal(rd, d)
+    q, d = plain_codes(x, 0, False)
+    assert torch.equal(col8, q) and torch.equal(cd, d)
+    for view, raw in ((row8, raw_r), (col8, raw_c)):     # nothing outside the matrix was written
+        view.fill_(0x5a)
+        assert raw.eq(0x5a).all()
+
+
+def test_quantise_infinities_and_nan(cfb):
+    x = normal((4, 256), 5)
+    x[0, 5] = float("inf")
+    x[1, 7] = float("nan")
+    x[2, 200] = float("-inf")
+    row8 = torch.empty((4, 256), dtype=torch.uint8, device="cuda")
+    rd = torch.empty((4, 2), device="cuda")
+    cfb.fp8_quantize_block128(x, row8, rd)
+    v = decode(row8, False) * rd.double().repeat_interleave(G, 1)
+    assert torch.isinf(rd[0, 0]) and v[0, :128].isnan().all()
+    assert v[1, 7].isnan() and torch.isfinite(v[1, :7]).all() and torch.isfinite(rd[1]).all()
+    assert torch.isfinite(v[2, :128]).all() and v[2, 128:].isnan().all()
+    clean = normal((4, 256), 5)
+    q, d = plain_codes(clean, 1, False)
+    assert torch.equal(row8[3], q[3]) and torch.equal(rd[3], d[3])
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (128, 128), (130, 260), (256, 1000), (5, 129), (3, 130, 140), (2, 128, 256), (4, 1, 16)])
+def test_quantise_weight_blocks_bit_exact(cfb, shape):
+    w = normal(shape, 11, 0.02)
+    w8 = torch.empty(shape, dtype=torch.uint8, device="cuda")
+    d = torch.empty((*shape[:-2], cdiv(shape[-2], G), cdiv(shape[-1], G)), device="cuda")
+    cfb.fp8_quantize_block128x128(w, w8, d)
+    for i in range(cdiv(shape[-2], G)):
+        for j in range(cdiv(shape[-1], G)):
+            part = w[..., i * G:(i + 1) * G, j * G:(j + 1) * G].float()
+            a = part.abs().amax((-2, -1), keepdim=True).clamp(min=1e-12)
+            q = (part * (448.0 / a.double()).float()).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+            assert torch.equal(w8[..., i * G:(i + 1) * G, j * G:(j + 1) * G], q)
+            assert torch.equal(d[..., i, j], (a.double() / 448.0).float()[..., 0, 0])
+
+
+# expf is off by 2 units (2^-23 each), the sigmoid's sum and division by one rounding each, then two products
+SWIGLU_SLACK = 8 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 14336), (5, 130), (129, 384), (300, 1001)])
+def test_swiglu_quantise(cfb, rows, cols):
+    gu = normal((rows, 2 * cols), 21, 2.0)
+    gate, up = gu[:, :cols], gu[:, cols:]
+    row8 = torch.empty((rows, cols), dtype=torch.uint8, device="cuda")
+    rd = cfb.block128_row_descale(rows, cols)
+    col8 = torch.empty_like(row8)
+    cd = torch.empty((cdiv(rows, G), cols), device="cuda")
+    cfb.swiglu_quantize_block128(gate, up, row8, rd, col8, cd)
+    v = gate.double() * torch.sigmoid(gate.double()) * up.double()
+    check_groups(row8, rd, v, 1, False, SWIGLU_SLACK)
+    check_groups(col8, cd, v, 0, False, SWIGLU_SLACK)
+    only = torch.empty_like(row8)
+    cfb.swiglu_quantize_block128(gate, up, only, rd.clone())
+    assert torch.equal(only, row8)
+
+
+@pytest.mark.parametrize("e5m2", [False, True])
+@pytest.mark.parametrize("rows,cols", [(1, 128), (129, 384), (300, 1024)])
+def test_swiglu_gradient_quantise(cfb, rows, cols, e5m2):
+    gu, dh = normal((rows, 2 * cols), 31, 2.0), normal((rows, cols), 32, 1e-3)
+    gate, up = gu[:, :cols], gu[:, cols:]
+    row8 = torch.empty((rows, 2 * cols), dtype=torch.uint8, device="cuda")
+    rd = cfb.block128_row_descale(rows, 2 * cols)
+    col8 = torch.empty_like(row8)
+    cd = torch.empty((cdiv(rows, G), 2 * cols), device="cuda")
+    cfb.swiglu_backward_quantize_block128(gate, up, dh, row8, rd, col8, cd, is_e5m2=e5m2)
+    g, u, d = gate.double().requires_grad_(), up.double().requires_grad_(), dh.double()
+    (g * torch.sigmoid(g) * u).backward(d)               # 64-bit differentiation of the definition
+    v = torch.cat([g.grad, u.grad], 1)
+    # 1 + gate (1 - sig): where the two terms cancel (gate near -1.28) the error is relative to the terms, each below 1.3
+    s = torch.sigmoid(gate.double())
+    absolute = torch.cat([(d * u.detach()).abs() * s * (1.0 + (gate.double() * (1 - s)).abs()), u.grad.abs()], 1) * SWIGLU_SLACK
+    for codes, scale, dim in ((row8, rd, 1), (col8, cd, 0)):
+        a, per = groups64(v, dim)
+        _, per_abs = groups64(absolute, dim)
+        assert (scale.double() - per / FMAX[e5m2]).abs().le((per_abs + 2 * U * per) / FMAX[e5m2]).all()
+        want = v / a * FMAX[e5m2]
+        bound = torch.maximum(want.abs() * HALF[e5m2], torch.full_like(want, TINY[e5m2])) * (1 + 2.0 ** -10)
+        bound = bound + absolute / a * FMAX[e5m2] + want.abs() * (4 * U + SWIGLU_SLACK)
+        assert (decode(codes, e5m2) - want).abs().le(bound).all()
+
+
+# ---------------------------------------------------------------- residual + norm
+NORM_SHAPES = [(1, 4096), (3, 1), (5, 100), (2, 129), (65, 512), (33, 1000), (7, 4100), (4, 8193), (3, 16384), (700, 2048)]
+
+
+def norm64(h, gain, eps):
+    h = h.double()
+    rms = (h.square().mean(1) + eps).sqrt()
+    return h / rms[:, None] * gain.double(), rms
+
+
+@pytest.mark.parametrize("rows,H", NORM_SHAPES)
+@pytest.mark.parametrize("residual", [True, False])
+def test_add_rmsnorm_quantise(cfb, rows, H, residual):
+    eps = 1e-5
+    x, r, gain = normal((rows, H), 41), normal((rows, H), 42, 3.0), normal((H,), 43)
+    h = torch.empty_like(x) if residual else None
+    rms, normed = torch.empty(rows, device="cuda"), torch.empty_like(x)
+    out8 = torch.empty((rows, H), dtype=torch.uint8, device="cuda")
+    d = cfb.block128_row_descale(rows, H)
+    cfb.add_rmsnorm_quantize_block128(x, r if residual else None, gain, h, rms, normed, out8, d, eps=eps)
+    want_h = (x.float() + r.float()).to(torch.bfloat16) if residual else x
+    if residual:
+        assert torch.equal(h, want_h)                    # one fp32 addition, one rounding
+    y, rms64 = norm64(want_h, gain, eps)
+    # sum of squares: at most 32 products per thread in a row, 5 + 32 additions behind them; root, division and two products
+    slack = (32 + 37 + 4) * U
+    assert (rms.double() - rms64).abs().le(slack * rms64).all()
+    assert (normed.double() - y).abs().le((2.0 ** -8 + slack) * y.abs() + 1e-38).all()
+    check_groups(out8, d, y, 1, False, slack)
+    # in place: h may be the residual, or x; the codes alone and the bf16 row alone are the same
+    for into in ("r", "x"):
+        xx, rr = x.clone(), r.clone()
+        o2, d2 = torch.empty_like(out8), torch.empty((rows, cdiv(H, G)), device="cuda")
+        if residual:
+            cfb.add_rmsnorm_quantize_block128(xx, rr, gain, rr if into == "r" else xx, None, None, o2, d2, eps=eps)
+            assert torch.equal(rr if into == "r" else xx, want_h)
+        else:
+            cfb.add_rmsnorm_quantize_block128(xx, None, gain, None, None, None, o2, d2, eps=eps)
+        assert torch.equal(o2, out8) and torch.equal(d2, d)
+    n2 = torch.empty_like(x)
+    cfb.add_rmsnorm_quantize_block128(want_h, None, gain, None, None, n2, eps=eps)
+    assert torch.equal(n2, normed)
+
+
+def test_add_rmsnorm_zero_rows_and_row_of_zeros(cfb):
+    gain = normal((256,), 1)
+    x = torch.zeros((2, 256), dtype=torch.bfloat16, device="cuda")
+    out8, d = torch.full((2, 256), 7, dtype=torch.uint8, device="cuda"), torch.empty((2, 2), device="cuda")
+    cfb.add_rmsnorm_quantize_block128(x, None, gain, None, None, None, out8, d)
+    assert (decode(out8, False) == 0).all() and torch.equal(d, (torch.full_like(d, 1e-12).double() / 448.0).float())
+    cfb.add_rmsnorm_quantize_block128(x[:0], None, gain, None, None, None, out8[:0], d[:0])
+
+
+def grad64(dy, h, gain, rms, dh):
+    dy, xh, g = dy.double(), h.double() / rms.double()[:, None], gain.double()
+    u = dy * g
+    dx = (u - xh * (u * xh).mean(1, keepdim=True)) / rms.double()[:, None]
+    return dx + (0 if dh is None else dh.double()), (dy * xh).sum(0)
+
+
+@pytest.mark.parametrize("rows,H", NORM_SHAPES + [(1500, 256)])
+@pytest.mark.parametrize("with_dh", [True, False])
+def test_add_rmsnorm_gradient(cfb, rows, H, with_dh):
+    eps = 1e-5
+    h, gain, dy = normal((rows, H), 51, 2.0), normal((H,), 52), normal((rows, H), 53, 1e-2)
+    dh = normal((rows, H), 54, 1e-2) if with_dh else None
+    rms = (h.double().square().mean(1) + eps).sqrt().float()
+    dx, dg = torch.empty_like(h), torch.full((H,), 3.0, device="cuda")
+    scratch = torch.full((cfb.add_rmsnorm_backward_scratch_floats(rows, H),), float("nan"), device="cuda")
+    cfb.add_rmsnorm_backward(dy, h, gain, rms, dh, dx, dg, scratch)
+    want_dx, want_dg = grad64(dy, h, gain, rms, dh)
+    # dx: bf16 rounding of the result; the mean is a sum of H products with the error of its absolute terms
+    xh = (h.double() / rms.double()[:, None]).abs()
+    u = (dy.double() * gain.double()).abs()
+    terms = (u + xh * (u * xh).mean(1, keepdim=True)) / rms.double()[:, None] + (0 if dh is None else dh.double().abs())
+    assert (dx.double() - want_dx).abs().le(2.0 ** -8 * want_dx.abs() + (32 + 37 + 8) * U * terms + 1e-38).all()
+    # dgain: per block at most rows / blocks products in a row, then at most 592 / 32 + 32 partial sums
+    depth = cdiv(rows, 148) + 19 + 32 + 4
+    assert (dg.double() - want_dg).abs().le(depth * U * (dy.double() * h.double() / rms.double()[:, None]).abs().sum(0)).all()
+    # accumulated on top; the same bits on every call; in place of either gradient; without the gain's gradient
+    dg2 = dg.clone()
+    into = dy.clone()
+    cfb.add_rmsnorm_backward(into, h, gain, rms, dh, into, dg2, scratch, accumulate_dscale=True)
+    assert torch.equal(into, dx) and torch.equal(dg2, dg + dg)
+    if with_dh:
+        into = dh.clone()
+        cfb.add_rmsnorm_backward(dy, h, gain, rms, into, into)
+        assert torch.equal(into, dx)
+
+
+def test_add_rmsnorm_gradient_against_differences(cfb):
+    """A directional derivative of sum(c * y(h)) in 64 bits against the kernel's gradient."""
+    rows, H, eps = 4, 512, 1e-5
+    h, gain, c, t = normal((rows, H), 61), normal((H,), 62), normal((rows, H), 63), normal((rows, H), 64).double()
+    tg = normal((H,), 65).double()
+    rms = norm64(h, gain, eps)[1].float()
+    dx, dg = torch.empty_like(h), torch.empty(H, device="cuda")
+    scratch = torch.empty(cfb.add_rmsnorm_backward_scratch_floats(rows, H), device="cuda")
+    cfb.add_rmsnorm_backward(c, h, gain, rms, None, dx, dg, scratch)
+
+    def f(e, eg):
+        hh, g = h.double() + e * t, gain.double() + eg * tg
+        return (c.double() * hh / (hh.square().mean(1, keepdim=True) + eps).sqrt() * g).sum()
+    s = 1e-5
+    dh_num, dg_num = (f(s, 0) - f(-s, 0)) / (2 * s), (f(0, s) - f(0, -s)) / (2 * s)
+    # dx is rounded to bf16: 2^-8 of every term; the difference quotient is good to s^2 and 1e-16 / s of the sum
+    tol = 2.0 ** -8 * (dx.double() * t).abs().sum() + 1e-6 * (c.double() * t).abs().sum()
+    assert (dh_num - (dx.double() * t).sum()).abs() <= tol
+    assert (dg_num - (dg.double() * tg).sum()).abs() <= 1e-5 * (dg.double() * tg).abs().sum()
+
+
+# ---------------------------------------------------------------- products
+def coded(rows, cols, seed, rows_per, cols_per, e5m2=False, std=1.0):
+    """Random codes (finite, over the whole range of the type) with a pitch that is a multiple of 16, and random descales."""
+    v = (torch.randn((rows, cols), generator=gen(seed), device="cuda") * std * 60).clamp(-FMAX[e5m2], FMAX[e5m2])
+    buf = torch.full((rows, cdiv(cols, 16) * 16), 0x7f, dtype=torch.uint8, device="cuda")     # NaN behind the columns: not to be read
+    buf[:, :cols] = v.to(TYPE[e5m2]).view(torch.uint8)
+    d = torch.rand((cdiv(rows, rows_per), cdiv(cols, cols_per)), generator=gen(seed + 1), device="cuda") * 0.02 + 1e-4
+    return buf[:, :cols], d
+
+
+def value64(codes, d, e5m2, rows_per, cols_per):
+    R, C = codes.shape
+    d = d.double().repeat_interleave(rows_per, 0)[:R].repeat_interleave(cols_per, 1)[:, :C]
+    return decode(codes, e5m2) * d
+
+
+def check_product(out, a, b, K, before=None):
+    """out = a . b (64 bits) up to fp32 sums and one rounding to out's type."""
+    want, mag = a @ b, a.abs() @ b.abs()
+    if before is not None:
+        want, mag = want + before, mag + before.abs()
+    # a block's 128 products are exact and added in fp32 (one unit of 2^-23 each at most); then per block the two scales'
+    # product, its product with the block and one addition
+    fp32 = (128 * 2 + 3 * cdiv(K, G) + 2) * U
+    half = 2.0 ** -8 if out.dtype == torch.bfloat16 else U
+    err = (out.double() - want).abs()
+    assert torch.isfinite(out).all()
+    bound = half * want.abs() + fp32 * mag
+    assert err.le(bound).all(), float((err / bound.clamp(min=1e-300)).max())
+
+
+NT_SHAPES = [(1, 1, 1), (1, 4096, 4096), (2, 100, 200), (16, 256, 128), (17, 129, 384), (33, 520, 1000), (64, 384, 2048),
+             (100, 128, 144), (128, 1000, 640), (129, 256, 128), (200, 64, 100), (300, 520, 1000), (513, 260, 272),
+             (777, 1000, 520), (512, 512, 4096), (1100, 2304, 1024)]
+
+
+@pytest.mark.parametrize("M,N,K", NT_SHAPES)
+def test_product_nt(cfb, ctx, M, N, K):
+    A, da = coded(M, K, M + N, 1, G)
+    B, db = coded(N, K, M + K, G, G, std=0.5)
+    out = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+    ctx.poll_status()
+    a, b = value64(A, da, False, 1, G), value64(B, db, False, G, G).t()
+    check_product(out, a, b, K)
+    # fp32 output, stored and added to; descales with the rows next to each other; the same sums
+    f = torch.full((M, N), 5.0, device="cuda")
+    cfb.gemm_fp8_block128_nt(ctx, A, da.t().contiguous().t(), B, db, f)
+    check_product(f, a, b, K)
+    assert torch.equal(f.to(torch.bfloat16), out)
+    g = f.clone()
+    cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, g, accumulate=True)
+    assert torch.equal(g, f + f)
+    c = normal((M, N), 9, 10.0)
+    c0 = c.clone()
+    cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, c, accumulate=True)
+    assert torch.equal(c, (c0.float() + f).to(torch.bfloat16))
+    ctx.poll_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 520), (130, 260, 272), (600, 300, 400)])
+def test_product_nt_types_row_groups_and_pitches(cfb, ctx, M, N, K):
+    A, da = coded(M, K, 1, 1, G, e5m2=True)
+    B, db = coded(N, K, 2, 1, G)
+    a, b = value64(A, da, True, 1, G), value64(B, db, False, 1, G).t()
+    for pad, offset in ((0, 0), (1, 0), (8, 8), (3, 1)):
+        out, raw = pitched(M, N, torch.bfloat16, pad, offset)
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out, a_is_e5m2=True)
+        check_product(out, a, b, K)
+        out.copy_(torch.full((), 0x5a5a, dtype=torch.int16, device="cuda").view(torch.bfloat16))
+        assert raw.eq(0x5a).all()                        # nothing between or behind the rows was written
+        f, raw = pitched(M, N, torch.float32, pad, offset)
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, f, a_is_e5m2=True)
+        check_product(f, a, b, K)
+        f.copy_(torch.full((), 0x5a5a5a5a, dtype=torch.int32, device="cuda").view(torch.float32))
+        assert raw.eq(0x5a).all()
+    ctx.poll_status()
+
+
+def test_product_scale_extremes(cfb, ctx):
+    """Scales far apart between blocks, zero scales, and a NaN or infinite scale that reaches its own row or column only."""
+    for M in (8, 300):
+        N, K = 384, 512
+        A, da = coded(M, K, 3, 1, G)
+        B, db = coded(N, K, 4, G, G)
+        da[:, 1] *= 1e6
+        da[:, 2] = 0.0
+        db[1, 3] = 0.0
+        out = torch.empty((M, N), device="cuda")
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+        check_product(out, value64(A, da, False, 1, G), value64(B, db, False, G, G).t(), K)
+        da[5, 0], db[2, 3] = float("nan"), float("inf")
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+        assert out[5].isnan().all() and not torch.isfinite(out[:, 256:]).any()
+        rest = torch.ones(M, dtype=torch.bool, device="cuda")
+        rest[5] = False
+        check_product(out[rest][:, :256], value64(A, da, False, 1, G)[rest], value64(B, db, False, G, G)[:256].t(), K)
+
+
+@pytest.mark.parametrize("counts,gap,tail", [([5, 0, 130, 1], 0, 3), ([300, 257, 0, 0, 40], 2, 0), ([0, 0], 0, 4), ([1], 0, 0),
+                                             ([700, 600, 513], 1, 9), ([3] * 130, 0, 1)])
+@pytest.mark.parametrize("N,K", [(256, 256), (200, 520)])
+def test_product_grouped(cfb, ctx, counts, gap, tail, N, K):
+    E = len(counts)
+    offsets = np.cumsum([0] + [c + gap for c in counts[:-1]])
+    T = int(offsets[-1]) + counts[-1] + tail
+    A, da = coded(T, K, 5, 1, G)
+    stack = [coded(N, K, 100 + 2 * e, G, G) for e in range(E)]
+    B = torch.stack([torch.nn.functional.pad(s[0], (0, -K % 16)) for s in stack])[..., :K]
+    db = torch.stack([s[1] for s in stack])
+    ct = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    ot = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    out, raw = pitched(T, N, torch.bfloat16, 8)
+    cfb.gemm_fp8_block128_nt_grouped(ctx, ct, ot, A, da, B, db, out)
+    ctx.poll_status()
+    a = value64(A, da, False, 1, G)
+    for e, (o, n) in enumerate(zip(offsets, counts)):
+        if n:
+            check_product(out[o:o + n], a[o:o + n], value64(B[e], db[e], False, G, G).t(), K)
+            out[o:o + n] = torch.full((), 0x5a5a, dtype=torch.int16, device="cuda").view(torch.bfloat16)
+    assert raw.eq(0x5a).all()                            # rows of no group, and everything between the rows, as they were
+
+
+def test_product_grouped_counts_that_leave_the_buffer(cfb, ctx):
+    """Device counts and offsets are not trusted: a group is cut to the buffer, one that starts outside is skipped."""
+    T, N, K, E = 140, 256, 256, 4
+    A, da = coded(T, K, 5, 1, G)
+    stack = [coded(N, K, 200 + 2 * e, G, G) for e in range(E)]
+    B, db = torch.stack([s[0] for s in stack]), torch.stack([s[1] for s in stack])
+    out, raw = pitched(T, N, torch.bfloat16, 0)
+    cfb.gemm_fp8_block128_nt_grouped(ctx, torch.tensor([10, 1000, 5, -7], dtype=torch.int32, device="cuda"),
+                                     torch.tensor([0, 20, 5000, 12], dtype=torch.int32, device="cuda"), A, da, B, db, out)
+    ctx.poll_status()
+    a = value64(A, da, False, 1, G)
+    check_product(out[:10], a[:10], value64(B[0], db[0], False, G, G).t(), K)
+    check_product(out[20:], a[20:], value64(B[1], db[1], False, G, G).t(), K)
+    assert raw.view(torch.bfloat16)[10 * N:20 * N].view(torch.int16).eq(0x5a5a).all()
+    assert raw[T * N * 2:].eq(0x5a).all()
+
+
+@pytest.mark.parametrize("e5m2", [False, True])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 1), (100, 200, 130), (300, 128, 520), (513, 1000, 256), (700, 272, 1100), (512, 512, 4096)])
+def test_product_nn(cfb, ctx, M, N, K, e5m2):
+    A, da = coded(M, K, 6, 1, G, e5m2=e5m2)
+    B, db = coded(K, N, 7, G, G)
+    out = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_nn(ctx, A, da, B, db, out, a_is_e5m2=e5m2)
+    ctx.poll_status()
+    a, b = value64(A, da, e5m2, 1, G), value64(B, db, False, G, G)
+    check_product(out, a, b, K)
+    f = torch.zeros((M, N), device="cuda")
+    cfb.gemm_fp8_block128_nn(ctx, A, da, B, db, f, a_is_e5m2=e5m2, accumulate=True)
+    assert torch.equal(f.to(torch.bfloat16), out)
+
+
+@pytest.mark.parametrize("xe,ye", [(False, True), (False, False), (True, False)])
+@pytest.mark.parametrize("M,N,T", [(16, 16, 1), (256, 300, 100), (100, 520, 130), (513, 260, 640), (1000, 272, 1100), (512, 768, 4096)])
+def test_product_dw(cfb, ctx, M, N, T, xe, ye):
+    X, dx = coded(T, M, 8, G, 1, e5m2=xe)
+    Y, dy = coded(T, N, 9, G, 1, e5m2=ye)
+    f = torch.full((M, N), 2.0, device="cuda")
+    cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, f, x_is_e5m2=xe, dy_is_e5m2=ye)
+    ctx.poll_status()
+    x, y = value64(X, dx, xe, G, 1).t(), value64(Y, dy, ye, G, 1)
+    check_product(f, x, y, T)
+    g = f.clone()
+    cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, g, x_is_e5m2=xe, dy_is_e5m2=ye, accumulate=True)
+    assert torch.equal(g, f + f)
+    h = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_dw(ctx, X, dx.t().contiguous().t(), Y, dy.t().contiguous().t(), h, x_is_e5m2=xe, dy_is_e5m2=ye)
+    assert torch.equal(h, f.to(torch.bfloat16))
+    c = normal((M, N), 10)
+    c0 = c.clone()
+    cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, c, x_is_e5m2=xe, dy_is_e5m2=ye, accumulate=True)
+    assert torch.equal(c, (c0.float() + f).to(torch.bfloat16))
+
+
+def test_empty_sizes_do_nothing(cfb, ctx):
+    A, da = coded(4, 256, 1, 1, G)
+    B, db = coded(128, 256, 2, G, G)
+    cfb.gemm_fp8_block128_nt(ctx, A[:0], da[:0], B, db, torch.empty((0, 128), dtype=torch.bfloat16, device="cuda"))
+    x = normal((0, 256), 1)
+    cfb.fp8_quantize_block128(x, torch.empty((0, 256), dtype=torch.uint8, device="cuda"), torch.empty((0, 2), device="cuda"))
+    dg = torch.ones(256, device="cuda")
+    cfb.add_rmsnorm_backward(x, x, normal((256,), 1), torch.empty(0, device="cuda"), None, x, dg, torch.empty(0, device="cuda"))
+    assert dg.eq(0).all()
+    cfb.add_rmsnorm_backward(x, x, normal((256,), 1), torch.empty(0, device="cuda"), None, x, dg.fill_(1), torch.empty(0, device="cuda"),
+                             accumulate_dscale=True)
+    assert dg.eq(1).all()
