@@ -7,10 +7,11 @@
 // warps fold each finished block into fp32 registers, acc += (da db) * block, while the tensor cores fill the other TMEM
 // buffer with the next block. Both operands' scales are arbitrary fp32 numbers (no power-of-two restriction).
 //
-// Wide form (k_gemm_b128): tiles of 256 x 256 per CTA pair (cta_group::2) or 128 x 256 per CTA, persistent, 320 threads:
-//   warp 0      TMA producer (one elected lane)
-//   warp 1      TMEM allocator + MMA issuer (one elected lane)
-//   warps 2..9  promotion + epilogue: each owns 32 rows x 128 columns of the CTA's 128 x 256 tile in 128 registers a thread
+// Wide form (k_gemm_b128): tiles of 256 x 256 per CTA pair (cta_group::2) or 128 x 256 per CTA, persistent, 384 threads:
+//   warp 0       TMA producer (one elected lane)
+//   warps 1, 3   MMA issuers for even and odd blocks (one elected lane each); warp 1 owns the TMEM allocation
+//   warp 2       scales: global memory -> shared-memory ring
+//   warps 4..11  promotion + epilogue: each owns 32 rows x 128 columns of the CTA's 128 x 256 tile in 128 registers a thread
 // Per block of 128 the MMAs of a CTA need 512 clocks; the promotion needs 64 packed multiply-adds per thread and two warps
 // per scheduler, 128 issue slots, and 128 KB of TMEM reads: it hides behind the MMAs.
 //
@@ -35,20 +36,31 @@ using namespace tc;
 constexpr int BM = 128;                 // rows of A / C per CTA (TMEM lanes)
 constexpr int BN = 256;                 // output columns per tile
 constexpr int SB = 128;                 // elements of K that share a scale == BK
-constexpr int NUM_THREADS = 320;
+constexpr int NUM_THREADS = 384;        // warpgroup 0: producer, two MMA issuers, scales; warpgroups 1 and 2: promotion + epilogue
 constexpr int EPI_WARPS = 8;
+// Registers: the launch gives every thread kLaunchRegs; warpgroup 0 hands most of its share to the two others, which hold 128
+// accumulators a thread. 56 x 128 + 224 x 256 = 168 x 384: the shares add up to what the launch has (the host checks that).
+constexpr int kLaunchRegs = 168, kLeanRegs = 56, kWideRegs = 224;
+static_assert(kLeanRegs * 128 + kWideRegs * 256 <= kLaunchRegs * NUM_THREADS, "register shares");
 constexpr int TMEM_COLS = 512;          // two 128x256 fp32 block sums per CTA
 constexpr int C_STAGING = EPI_WARPS * C_BOX_BYTES;
+// Scales on their way from global memory: a ring of blocks, each with the 128 row scales and the column scales (256, or one
+// per 128 columns) of the CTA's tile, filled by a warp of its own with 4-byte asynchronous copies several blocks ahead. A
+// scale's first use misses L1 and often L2 (another line for every block of K): loaded by the promotion warps one block
+// ahead, or copied by them several blocks ahead, the scales took more of their time than the promotion itself.
+constexpr int SCALE_DEPTH = 8;
+constexpr int SCALE_ENTRY = BM + BN;                       // floats
+constexpr int SCALE_RING = SCALE_DEPTH * SCALE_ENTRY * 4;
 
 template <bool PAIR>
 struct Cfg {
     static constexpr int B_ROWS = PAIR ? 128 : 256;
-    static constexpr int STAGES = PAIR ? 6 : 4;
+    static constexpr int STAGES = PAIR ? 5 : 3;
     static constexpr int A_STAGE = BM * BK;
     static constexpr int B_STAGE = B_ROWS * BK;
     static constexpr int TILE_M = PAIR ? 256 : 128;
     static constexpr int RING = STAGES * (A_STAGE + B_STAGE);
-    static constexpr int SMEM_BYTES = RING + C_STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+    static constexpr int SMEM_BYTES = RING + C_STAGING + SCALE_RING + 1024 /*alignment slack*/ + 512 /*barriers*/;
 };
 
 enum OutKind { OUT_BF16 = 0, OUT_F32 = 1, OUT_F32_ADD = 2, OUT_BF16_ADD = 3 };
@@ -98,6 +110,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
+// 4 bytes from global to shared memory without a register; zero where !ok (src is then not read, but has to be an address).
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+// Arrives on the barrier once this thread's earlier asynchronous copies have landed (the count includes every such thread).
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint16_t to_bf16_bits(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 
 __device__ __forceinline__ void store_value(const Params& p, long long row, long long col, float v) {
@@ -109,6 +130,13 @@ __device__ __forceinline__ void store_value(const Params& p, long long row, long
         uint16_t* c = static_cast<uint16_t*>(p.C) + i;
         *c = to_bf16_bits(bf16_bits_to_f32(*c) + v);
     }
+}
+
+// Frees a TMEM buffer on the leader's barrier. The default (CTA-scope) release is enough: what is handed over is TMEM, whose
+// reads tcgen05.wait::ld and the tcgen05 fence have completed. A cluster-scope release costs a memory barrier that waits for
+// the scale loads in flight, once per block of K.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------
@@ -183,11 +211,14 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const uint32_t smem_a = base;
     const uint32_t smem_b = base + STAGES * A_STAGE;
     const uint32_t smem_c = smem_b + STAGES * B_STAGE;
-    const uint32_t bars = smem_c + C_STAGING;
-    const uint32_t full_bar = bars, empty_bar = bars + 8 * STAGES;
-    const uint32_t tfull_bar = bars + 16 * STAGES, tempty_bar = tfull_bar + 16, drain_bar = tempty_bar + 16;
+    const uint32_t bars = smem_c + C_STAGING + SCALE_RING;
+    const uint32_t full_bar = bars, done_bar = bars + 8 * STAGES;      // per stage: operands there / block multiplied
+    const uint32_t tempty_bar = bars + 16 * STAGES, drain_bar = tempty_bar + 16;
+    const uint32_t sfull_bar = drain_bar + 16, sempty_bar = sfull_bar + 8 * SCALE_DEPTH;
     uint8_t* gen = smem_raw + (base - raw);
-    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C_STAGING + 16 * STAGES + 48);
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C_STAGING + SCALE_RING + 16 * STAGES + 48 + 16 * SCALE_DEPTH);
+    const uint32_t ring = smem_c + C_STAGING;
+    const float* ring_f = reinterpret_cast<const float*>(gen + C::RING + C_STAGING);
     volatile int* s_abort = reinterpret_cast<volatile int*>(const_cast<uint32_t*>(s_tmem) + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -199,13 +230,16 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar + 8 * s, 1);
-            mbar_init(empty_bar + 8 * s, 1);
+            mbar_init(done_bar + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
-            mbar_init(tfull_bar + 8 * a, 1);
             mbar_init(tempty_bar + 8 * a, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+            mbar_init(drain_bar + 8 * a, 1);
         }
-        mbar_init(drain_bar, 1);
+        for (int e = 0; e < SCALE_DEPTH; ++e) {
+            mbar_init(sfull_bar + 8 * e, 32);                // the lanes of the scale warp, each when its copies have landed
+            mbar_init(sempty_bar + 8 * e, EPI_WARPS);
+        }
         s_abort[0] = 0;
         s_abort[1] = 0;                                      // stays 0: abort source for the drain waits
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -246,10 +280,13 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int total_tiles = m_blocks * ((p.N + BN - 1) / BN);
     const int k_iters = (p.K + BK - 1) / BK;
 
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (both CTAs of a pair)
         if (lane == 0) {
-            int it = 0;
+            int it = 0, s = 0;
+            uint32_t phase = 1;                              // the ring starts out empty
             bool ok = true;
             const uint32_t full_dst = PAIR ? mapa(full_bar, 0) : full_bar;
             for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
@@ -257,8 +294,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 const int a_row = tc_.row0 + static_cast<int>(cta_rank) * BM;
                 const int b_col = tc_.n0 + static_cast<int>(cta_rank) * C::B_ROWS;       // rank is 0 in the single form
                 for (int kb = 0; kb < k_iters; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (!mbar_wait(empty_bar + 8 * s, ((it / STAGES) & 1) ^ 1, s_abort)) { ok = false; break; }
+                    if (!mbar_wait(done_bar + 8 * s, phase, s_abort)) { ok = false; break; }
                     // K-major operand: x runs along K. MN-major operand ([K, rows] in memory): x runs along the rows, the
                     // box rows are K (pair form only: a CTA's share is one box of 128 bytes)
                     const int ax = p.a_mn ? a_row : kb * BK, ay = p.a_mn ? kb * BK : a_row;
@@ -272,6 +308,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         tma_load_2d(smem_a + s * A_STAGE, &map_a, full_bar + 8 * s, ax, ay);
                         tma_load_2d(smem_b + s * B_STAGE, &map_b, full_bar + 8 * s, bx, by);
                     }
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
             if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x500 | 1); }
@@ -280,127 +317,150 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     mbar_wait(full_bar + 8 * (j % STAGES), (j / STAGES) & 1, s_abort + 1 /*never set*/, DRAIN_NS);
             }
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    } else if (warp == 1 || warp == 3) {
+        // ------------------------------------------------------------ MMA issuers (leader CTA only)
+        // Warp 1 issues the even blocks, warp 3 the odd ones, each into its own TMEM buffer: the two sequences do not depend on
+        // each other, and while one thread waits for barriers and commits, the other one's MMAs keep the tensor cores fed.
+        // One issuer for both left them idle for half of the time (1030 clocks a block where its MMAs take 500).
         if (lane == 0 && leader) {
+            const int mine = warp >> 1;                      // 0: even, 1: odd
+            const int blocks = unit < total_tiles ? ((total_tiles - unit - 1) / n_units + 1) * k_iters : 0;
             const uint32_t idesc = make_idesc(p.a_e5m2, p.b_e5m2, TM, BN, p.a_mn, p.b_mn);
             // one MMA covers 32 of K: 32 bytes further inside the swizzle atom of a K-major operand, 32 rows of 128 bytes
             // further in an MN-major one
             const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
-            int it = 0;
+            const uint32_t tmem_d = tmem_base + mine * BN, tempty = tempty_bar + 8 * mine;
+            int s = mine;
+            uint32_t phase = 0, t_phase = 1;
             bool ok = true;
-            for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
-                for (int kb = 0; kb < k_iters; ++kb, ++it) {
-                    const int s = it % STAGES, buf = it & 1;
-                    if (!mbar_wait(tempty_bar + 8 * buf, ((it >> 1) & 1) ^ 1, s_abort)) { ok = false; break; }
-                    if (!mbar_wait(full_bar + 8 * s, (it / STAGES) & 1, s_abort)) { ok = false; break; }
-                    tcgen05_fence_after();
-                    const uint64_t adesc = make_smem_desc(smem_a + s * A_STAGE);
-                    const uint64_t bdesc = make_smem_desc(smem_b + s * B_STAGE);
-                    const uint32_t tmem_d = tmem_base + buf * BN;
+            for (int it = mine; it < blocks; it += 2) {
+                if (!mbar_wait(tempty, t_phase, s_abort) || !mbar_wait(full_bar + 8 * s, phase, s_abort)) { ok = false; break; }
+                tcgen05_fence_after();
+                const uint64_t adesc = make_smem_desc(smem_a + s * A_STAGE);
+                const uint64_t bdesc = make_smem_desc(smem_b + s * B_STAGE);
 #pragma unroll
-                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                        if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
-                        else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
-                    }
-                    if (PAIR) {
-                        tcgen05_commit_pair(empty_bar + 8 * s);
-                        tcgen05_commit_pair(tfull_bar + 8 * buf);
-                    } else {
-                        tcgen05_commit(empty_bar + 8 * s);
-                        tcgen05_commit(tfull_bar + 8 * buf);
-                    }
+                for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                    if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                    else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
                 }
+                // the stage may be filled again, and the block's sums may be read (in both CTAs of a pair)
+                if (PAIR) tcgen05_commit_pair(done_bar + 8 * s); else tcgen05_commit(done_bar + 8 * s);
+                t_phase ^= 1u;
+                s += 2;
+                if (s >= STAGES) { s -= STAGES; phase ^= 1u; }
             }
             if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x600 | 1); }
             if (*s_abort || !ok) {
-                if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar) : "memory");
-                else tcgen05_commit(drain_bar);
-                mbar_wait(drain_bar, 0, s_abort + 1, DRAIN_NS);
+                if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar + 8 * mine) : "memory");
+                else tcgen05_commit(drain_bar + 8 * mine);
+                mbar_wait(drain_bar + 8 * mine, 0, s_abort + 1, DRAIN_NS);
             }
         }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ scales (both CTAs of a pair, their own rows)
+        int e = 0;
+        uint32_t phase = 1;                                  // the ring starts out empty
+        bool ok = true;
+        for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
+            const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
+            const int row = tc_.row0 + static_cast<int>(cta_rank) * BM + lane;
+            const float* sa = p.sa + row * p.sa_row;
+            const float* sb = p.sb + tc_.group * p.sb_group + (BVEC ? (tc_.n0 + lane) * p.sb_row : (tc_.n0 / SB + lane) * p.sb_row);
+            for (int kb = 0; kb < k_iters; ++kb) {
+                if (!mbar_wait(sempty_bar + 8 * e, phase, s_abort)) { ok = false; break; }
+                const uint32_t dst = ring + e * (SCALE_ENTRY * 4) + lane * 4;
+                // rows and columns outside of the product get scale 0 (their results are not stored)
+#pragma unroll
+                for (int q = 0; q < BM / 32; ++q) {
+                    const bool in = row + 32 * q < tc_.end;
+                    cp_async4(dst + 128 * q, in ? sa + 32 * q * p.sa_row : p.sa, in);
+                }
+                if (BVEC) {
+#pragma unroll
+                    for (int q = 0; q < BN / 32; ++q) {
+                        const bool in = tc_.n0 + lane + 32 * q < p.N;
+                        cp_async4(dst + 4 * BM + 128 * q, in ? sb + 32 * q * p.sb_row : p.sb, in);
+                    }
+                } else if (lane < BN / SB) {
+                    const bool in = tc_.n0 + lane * SB < p.N;
+                    cp_async4(dst + 4 * BM, in ? sb : p.sb, in);
+                }
+                cp_async_arrive(sfull_bar + 8 * e);
+                sa += p.sa_blk;
+                sb += p.sb_blk;
+                if (++e == SCALE_DEPTH) { e = 0; phase ^= 1u; }
+            }
+        }
+        if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xb00 | 1); }
+        cp_async_wait_all();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegs));
         // ------------------------------------------------------------ promotion + epilogue (both CTAs of a pair)
         const int quarter = warp & 3;                      // TMEM lanes this warp may read
-        const int half = (warp - 2) >> 2;                  // which 128 columns of the tile
+        const int half = (warp - 4) >> 2;                  // which 128 columns of the tile
         const uint32_t tempty_dst = PAIR ? mapa(tempty_bar, 0) : tempty_bar;
-        const uint32_t box = smem_c + static_cast<uint32_t>(warp - 2) * C_BOX_BYTES;
-        float* box_f = reinterpret_cast<float*>(gen + C::RING + (warp - 2) * C_BOX_BYTES);
+        const uint32_t box = smem_c + static_cast<uint32_t>(warp - 4) * C_BOX_BYTES;
+        float* box_f = reinterpret_cast<float*>(gen + C::RING + (warp - 4) * C_BOX_BYTES);
         const uint64_t store_policy = l2_policy_evict_first();
-        int it = 0;
+        int it = 0, e = 0, st = 0;                         // block, slot of its scales, its stage
+        uint32_t s_phase = 0, d_phase = 0;
         bool ok = true;
         for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
             const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
             const int warp_row = tc_.row0 + static_cast<int>(cta_rank) * BM + quarter * 32;
-            const int row = warp_row + lane;
             const int wcol = tc_.n0 + half * 128;          // first column of this warp
-            const bool live = row < tc_.end;
-            const float* sa = p.sa + (live ? row * p.sa_row : 0);
-            const float* sb = p.sb + tc_.group * p.sb_group;
-            // columns of this warp beyond N get scale 0 (their products are never stored)
-            if (!BVEC) sb += (wcol / SB) * p.sb_row;
-            const bool sb_ok = wcol < p.N;
             uint64_t acc[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) acc[j] = 0ull;
-            float sa_next = live ? __ldg(sa) : 0.0f;
-            float sb_next = 0.0f;
-            float cs[4];                                   // BVEC: lane l carries columns l, l+32, l+64, l+96 of the next block
-            if (BVEC) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = wcol + lane + 32 * q;
-                    cs[q] = c < p.N ? __ldg(sb + c * p.sb_row) : 0.0f;
-                }
-                if (lane == 0) bulk_wait_read_0();         // the box doubles as the scales' buffer: its last store has left
-                __syncwarp();
-            } else {
-                sb_next = sb_ok ? __ldg(sb) : 0.0f;
-            }
-            for (int kb = 0; kb < k_iters; ++kb, ++it) {
+            // The reads of TMEM run one chunk of 32 columns ahead of the arithmetic, over block boundaries too: while a chunk
+            // is folded in, the next one is on its way. A buffer goes back as soon as its last chunk is in registers.
+            const uint32_t tcol = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+            uint32_t v[2][32];
+            ok = mbar_wait(sfull_bar + 8 * e, s_phase, s_abort) && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
+            if (!ok) break;
+            tcgen05_fence_after();
+            tmem_ld32(tcol + (it & 1) * BN, v[0]);
+            for (int kb = 0; kb < k_iters; ++kb) {
                 const int buf = it & 1;
-                const float s_row = BVEC ? sa_next : sa_next * sb_next;
-                if (BVEC) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) box_f[buf * 128 + lane + 32 * q] = cs[q];
-                    __syncwarp();
-                }
-                if (kb + 1 < k_iters) {                    // the next block's scales are on their way during this one
-                    if (live) sa_next = __ldg(sa + (kb + 1) * p.sa_blk);
-                    if (BVEC) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int c = wcol + lane + 32 * q;
-                            if (c < p.N) cs[q] = __ldg(sb + c * p.sb_row + (kb + 1) * p.sb_blk);
-                        }
-                    } else if (sb_ok) {
-                        sb_next = __ldg(sb + (kb + 1) * p.sb_blk);
-                    }
-                }
-                if (!mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort)) { ok = false; break; }
-                tcgen05_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
+                const float* entry = ring_f + e * SCALE_ENTRY;
+                const float* cs = entry + BM + half * 128;
+                const float s_row = BVEC ? entry[quarter * 32 + lane] : entry[quarter * 32 + lane] * entry[BM + half];
                 const uint64_t s2 = pack_f2(s_row, s_row);
-                uint32_t v[2][16];
-                tmem_ld16(taddr, v[0]);
+                const uint32_t done = sempty_bar + 8 * e;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     tmem_ld_wait();
-                    if (c < 7) tmem_ld16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint64_t x = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
-                        if (BVEC) {
-                            const float2 b2 = *reinterpret_cast<const float2*>(box_f + buf * 128 + c * 16 + 2 * j);
-                            x = mul_f2(x, pack_f2(b2.x, b2.y));
+                    if (c < 3) {
+                        tmem_ld32(tcol + buf * BN + (c + 1) * 32, v[(c + 1) & 1]);
+                    } else {
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) mbar_arrive_remote(tempty_dst + 8 * buf); else mbar_arrive(tempty_bar + 8 * buf);
+                            if (!BVEC) mbar_arrive(done);
                         }
-                        acc[c * 8 + j] = fma_f2(x, s2, acc[c * 8 + j]);
+                        ++it;
+                        if (++e == SCALE_DEPTH) { e = 0; s_phase ^= 1u; }
+                        if (++st == STAGES) { st = 0; d_phase ^= 1u; }
+                        if (kb + 1 < k_iters) {
+                            ok = mbar_wait(sfull_bar + 8 * e, s_phase, s_abort) && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                            tmem_ld32(tcol + (it & 1) * BN, v[0]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        uint64_t x = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
+                        if (BVEC) x = mul_f2(x, *reinterpret_cast<const uint64_t*>(cs + c * 32 + 2 * j));
+                        acc[c * 16 + j] = fma_f2(x, s2, acc[c * 16 + j]);
                     }
                 }
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (PAIR) mbar_arrive_cluster(tempty_dst + 8 * buf); else mbar_arrive(tempty_bar + 8 * buf);
+                if (!ok) break;
+                if (BVEC) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(done);
                 }
             }
             if (!ok) break;
@@ -697,8 +757,22 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
+template <class K>
+int check_regs(K* kernel) {
+    cudaFuncAttributes a;
+    CF_CUDA(cudaFuncGetAttributes(&a, kernel));
+    if (a.numRegs < kLaunchRegs) {          // the warpgroups' shares would not add up: setmaxnreg.inc would wait for ever
+        set_error("k_gemm_b128 was built with %d registers a thread, its register split needs %d", a.numRegs, kLaunchRegs);
+        return CF_ERR_UNSUPPORTED;
+    }
+    return CF_OK;
+}
 template <bool PAIR>
 int set_smem() {
+    int rc = check_regs(k_gemm_b128<PAIR, false>);
+    if (rc == CF_OK) rc = check_regs(k_gemm_b128<PAIR, true>);
+    if (rc != CF_OK) return rc;
+
     cudaError_t e = cudaFuncSetAttribute(k_gemm_b128<PAIR, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_gemm_b128<PAIR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES);
     return e == cudaSuccess ? CF_OK : cuda_fail(e, "cudaFuncSetAttribute(k_gemm_b128)");
