@@ -20,7 +20,7 @@ namespace cf {
 namespace {
 
 constexpr int kMaxH = 16384;
-constexpr int kBwdBlocks = 592;             // 4 per SM: fixed, so that the order of the partial sums does not follow the device
+constexpr int kBwdBlocks = 148;             // per block that an SM holds: fixed, so that the order of the sums does not follow the device
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
     f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
@@ -129,27 +129,45 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
         const float rms = sqrtf(__fdiv_rn(total, static_cast<float>(p.H)) + p.eps);
         if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
         const float inv = __fdiv_rn(1.0f, rms);
+        float amax[NV];                                 // of the group of 128 that this half-warp holds in vector i
+        float y[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int vi = threadIdx.x + blockDim.x * i;
-            float f[8], g[8];
-            unpack8(v[i], f);
+            float g[8];
+            unpack8(v[i], y[i]);
             unpack8(vi < nv ? load8<VEC>(p.gain + vi * 8, p.H - vi * 8) : make_uint4(0u, 0u, 0u, 0u), g);
-            float a = 0.0f;
+            amax[i] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                f[e] = f[e] * inv * g[e];
-                a = fmaxf(a, fabsf(f[e]));
+                y[i][e] = y[i][e] * inv * g[e];
+                amax[i] = fmaxf(amax[i], fabsf(y[i][e]));
             }
-            if (p.normed && vi < nv) store8<VEC>(p.normed + base + vi * 8, pack8(f), p.H - vi * 8);
-            if (p.out8) {                               // kernel-uniform: the half-warp holds one group of 128
+            if (p.normed && vi < nv) store8<VEC>(p.normed + base + vi * 8, pack8(y[i]), p.H - vi * 8);
+        }
+        if (p.out8) {                                   // kernel-uniform
 #pragma unroll
-                for (int off = 8; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-                a = fmaxf(a, 1e-12f);
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], off));
+            }
+            // lane i of a half-warp divides for group i, the quotients are handed round
+            const int lane = threadIdx.x & 31, cg = lane & 15;
+            float mine = amax[0];
+#pragma unroll
+            for (int i = 1; i < NV; ++i)
+                if (cg == i) mine = amax[i];
+            mine = fmaxf(mine, 1e-12f);
+            const float scale = __fdiv_rn(448.0f, mine);
+            const int my_group = (threadIdx.x + blockDim.x * cg) / 16;
+            if (cg < NV && my_group * 16 < nv) p.descale[row * p.d_row + my_group * p.d_blk] = __fdiv_rn(mine, 448.0f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int vi = threadIdx.x + blockDim.x * i;
+                const float s = __shfl_sync(0xffffffffu, scale, (lane & 16) | i);
                 if (vi < nv) {
-                    const float s = __fdiv_rn(448.0f, a);
-                    const uint32_t q0 = cvt_fp8x4<false>(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
-                    const uint32_t q1 = cvt_fp8x4<false>(f[4] * s, f[5] * s, f[6] * s, f[7] * s);
+                    const uint32_t q0 = cvt_fp8x4<false>(y[i][0] * s, y[i][1] * s, y[i][2] * s, y[i][3] * s);
+                    const uint32_t q1 = cvt_fp8x4<false>(y[i][4] * s, y[i][5] * s, y[i][6] * s, y[i][7] * s);
                     uint8_t* o = p.out8 + row * p.ld_out8 + vi * 8;
                     if (VEC && p.vec8) {
                         *reinterpret_cast<uint2*>(o) = make_uint2(q0, q1);
@@ -158,7 +176,6 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
                         for (int e = 0; e < 8; ++e)
                             if (vi * 8 + e < p.H) o[e] = static_cast<uint8_t>((e < 4 ? q0 >> (8 * e) : q1 >> (8 * (e - 4))) & 0xffu);
                     }
-                    if ((threadIdx.x & 15) == 0) p.descale[row * p.d_row + (vi / 16) * p.d_blk] = __fdiv_rn(a, 448.0f);
                 }
             }
         }
@@ -176,9 +193,9 @@ struct NormGradParams {
     int rows, H;
 };
 
-// dx may be the same memory as dy or dh.
-template <int NV, bool VEC>
-__global__ void __launch_bounds__(512) k_add_rmsnorm_grad(const NormGradParams p) {
+// dx may be the same memory as dy or dh. PREFETCH: the next row's loads are issued before this row's barrier.
+template <int NV, bool VEC, int MAXT, bool PREFETCH>
+__global__ void __launch_bounds__(MAXT, MAXT <= 512 && PREFETCH ? 2 : 1) k_add_rmsnorm_grad(const NormGradParams p) {
     __shared__ float s_sum[2][32];
     const int nv = (p.H + 7) / 8;
     float dg[NV][8];
@@ -190,28 +207,34 @@ __global__ void __launch_bounds__(512) k_add_rmsnorm_grad(const NormGradParams p
 #pragma unroll
         for (int e = 0; e < 8; ++e) dg[i][e] = 0.0f;
     }
-    int par = 0;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
+    struct Row { uint4 dy[NV], h[NV], dh[NV]; float rms; };
+    auto load = [&](Row& r, long long row) {
         const long long base = row * p.H;
-        uint4 dy[NV], h[NV], dh[NV];
+        r.rms = p.rms[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int vi = threadIdx.x + blockDim.x * i;
-            dy[i] = h[i] = dh[i] = make_uint4(0u, 0u, 0u, 0u);
+            r.dy[i] = r.h[i] = r.dh[i] = make_uint4(0u, 0u, 0u, 0u);
             if (vi < nv) {
-                dy[i] = load8<VEC>(p.dy + base + vi * 8, p.H - vi * 8);
-                h[i] = load8<VEC>(p.h + base + vi * 8, p.H - vi * 8);
-                if (p.dh) dh[i] = load8<VEC>(p.dh + base + vi * 8, p.H - vi * 8);
+                r.dy[i] = load8<VEC>(p.dy + base + vi * 8, p.H - vi * 8);
+                r.h[i] = load8<VEC>(p.h + base + vi * 8, p.H - vi * 8);
+                if (p.dh) r.dh[i] = load8<VEC>(p.dh + base + vi * 8, p.H - vi * 8);
             }
         }
-        const float rms = p.rms[row];
-        const float inv = __fdiv_rn(1.0f, rms);
+    };
+    int par = 0;
+    Row r, next;
+    if (PREFETCH && blockIdx.x < p.rows) load(r, blockIdx.x);
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
+        if (!PREFETCH) load(r, row);
+        else if (row + gridDim.x < p.rows) load(next, row + gridDim.x);
+        const float inv = __fdiv_rn(1.0f, r.rms);
         float acc = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float a[8], b[8], g[8];
-            unpack8(dy[i], a);
-            unpack8(h[i], b);
+            unpack8(r.dy[i], a);
+            unpack8(r.h[i], b);
             unpack8(gain[i], g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -224,14 +247,15 @@ __global__ void __launch_bounds__(512) k_add_rmsnorm_grad(const NormGradParams p
         for (int i = 0; i < NV; ++i) {
             const int vi = threadIdx.x + blockDim.x * i;
             float a[8], b[8], g[8], d[8];
-            unpack8(dy[i], a);
-            unpack8(h[i], b);
+            unpack8(r.dy[i], a);
+            unpack8(r.h[i], b);
             unpack8(gain[i], g);
-            unpack8(dh[i], d);
+            unpack8(r.dh[i], d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e] = fmaf(fmaf(-b[e] * inv, mean, a[e] * g[e]), inv, d[e]);
-            if (vi < nv) store8<VEC>(p.dx + base + vi * 8, pack8(d), p.H - vi * 8);
+            if (vi < nv) store8<VEC>(p.dx + row * p.H + vi * 8, pack8(d), p.H - vi * 8);
         }
+        if (PREFETCH) r = next;
     }
     if (p.partial) {
         float* o = p.partial + static_cast<long long>(blockIdx.x) * p.H;
@@ -271,21 +295,26 @@ int threads_for(int nv, int per_thread) {
     return (t + 31) / 32 * 32;
 }
 
+// Vectors of 8 a thread holds. Forward: four; with few rows as few as possible, so that a row is spread over more threads (one
+// row of 4096: 512 threads). Gradient: one, which leaves registers for the next row's loads; four for rows beyond 8192 elements
+// (a block has 1024 threads at most).
+constexpr int kFwdVec = 4;
+constexpr int grad_vec(int H) { return H <= 8192 ? 1 : 4; }
+
 template <int NV, bool VEC>
 int launch_forward(const NormParams& p, cudaStream_t st) {
     const int t = threads_for((p.H + 7) / 8, NV);
-    int per_sm = 0;
-    CF_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_add_rmsnorm<NV, VEC>, t, 0));
-    long long grid = static_cast<long long>(sm_count()) * (per_sm < 1 ? 1 : per_sm);
-    if (grid > p.rows) grid = p.rows;
+    // resident blocks, two rounds of them at most: the rest of the rows is walked by the blocks
+    const long long most = static_cast<long long>(sm_count()) * (2048 / t < 16 ? 2048 / t : 16);
+    const long long grid = p.rows < most ? p.rows : most;
     k_add_rmsnorm<NV, VEC><<<static_cast<unsigned>(grid), t, 0, st>>>(p);
     CF_LAUNCH_CHECK("add_rmsnorm");
     return CF_OK;
 }
 
 int grad_blocks(int rows, int H) {
-    const int t = threads_for((H + 7) / 8, 4);
-    int b = kBwdBlocks / 4 * (t <= 128 ? 4 : t <= 256 ? 2 : 1);
+    const int t = threads_for((H + 7) / 8, grad_vec(H));
+    const int b = kBwdBlocks * (grad_vec(H) > 1 ? 1 : t <= 128 ? 8 : t <= 256 ? 4 : t <= 512 ? 2 : 1);
     return b < rows ? b : rows;
 }
 
@@ -324,8 +353,9 @@ int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_
     const bool vec = H % 8 == 0 && aligned(d_x, 16) && aligned(d_residual_or_null, 16) && aligned(d_scale, 16) &&
                      aligned(d_h_or_null, 16) && aligned(d_normed_or_null, 16);
     cudaStream_t st = as_stream(stream);
-    if (!vec) return launch_forward<4, false>(p, st);
-    return launch_forward<4, true>(p, st);
+    if (!vec) return launch_forward<kFwdVec, false>(p, st);
+    if (rows <= sm_count()) return H <= 8192 ? launch_forward<1, true>(p, st) : launch_forward<2, true>(p, st);
+    return launch_forward<kFwdVec, true>(p, st);
 }
 
 size_t cf_add_rmsnorm_backward_scratch_floats(int rows, int H) {
@@ -360,9 +390,17 @@ int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_sca
     p.partial = d_dscale_or_null ? d_scratch : nullptr;
     p.rows = rows; p.H = H;
     const bool vec = H % 8 == 0 && aligned(d_dy, 16) && aligned(d_h, 16) && aligned(d_scale, 16) && aligned(d_dh_or_null, 16) && aligned(d_dx, 16);
-    const int t = threads_for((H + 7) / 8, 4), blocks = grad_blocks(rows, H);
-    if (vec) k_add_rmsnorm_grad<4, true><<<blocks, t, 0, st>>>(p);
-    else k_add_rmsnorm_grad<4, false><<<blocks, t, 0, st>>>(p);
+    const int nv = grad_vec(H), t = threads_for((H + 7) / 8, nv), blocks = grad_blocks(rows, H);
+    if (nv == 1 && t <= 512) {
+        if (vec) k_add_rmsnorm_grad<1, true, 512, true><<<blocks, t, 0, st>>>(p);
+        else k_add_rmsnorm_grad<1, false, 512, true><<<blocks, t, 0, st>>>(p);
+    } else if (nv == 1) {
+        if (vec) k_add_rmsnorm_grad<1, true, 1024, true><<<blocks, t, 0, st>>>(p);
+        else k_add_rmsnorm_grad<1, false, 1024, true><<<blocks, t, 0, st>>>(p);
+    } else {
+        if (vec) k_add_rmsnorm_grad<4, true, 512, false><<<blocks, t, 0, st>>>(p);
+        else k_add_rmsnorm_grad<4, false, 512, false><<<blocks, t, 0, st>>>(p);
+    }
     CF_LAUNCH_CHECK("add_rmsnorm_grad");
     if (d_dscale_or_null) {
         k_sum_partials<<<(H + 31) / 32, 1024, 0, st>>>(d_scratch, blocks, H, d_dscale_or_null, accumulate_dscale);
