@@ -29,7 +29,7 @@ __all__ = [
     "block128_row_descale", "fp8_quantize_block128", "swiglu_quantize_block128", "swiglu_backward_quantize_block128", "fp8_quantize_block128x128",
     "add_rmsnorm_quantize_block128", "add_rmsnorm_backward", "add_rmsnorm_backward_scratch_floats",
     "gemm_fp8_block128_nt", "gemm_fp8_block128_nt_grouped", "gemm_fp8_block128_nn", "gemm_fp8_block128_dw",
-    "moe_grouped_expert_forward_fp8", "launch_count", "swiglu_mlp_fp8_rowwise", "MoeSwigluFp8", "FfnSwigluFp8",
+    "moe_grouped_expert_forward_fp8", "launch_count", "swiglu_mlp_fp8_rowwise", "MoeSwigluFp8", "FfnSwigluFp8", "Fp8Block128Weight", "FfnSwigluFp8Block128",
 ]
 
 
@@ -573,35 +573,46 @@ def moe_grouped_expert_forward_fp8(ctx, hidden, fcin_descale, fcin_is_e5m2, rout
 
 # ---------------------------------------------------------------- block-scaled FP8 (one scale per 128 values)
 BLOCK = 128
+_bf16, _u8, _f32, _i32 = torch.bfloat16, torch.uint8, torch.float32, torch.int32
 
 
-def _need(ok, what):
+def _refuse(what):
     """A call whose tensors do not fit together is refused before any pointer reaches the library."""
-    if not ok:
-        raise CanopyError(_capi.CF_ERR_INVALID_ARG, what)
+    raise CanopyError(_capi.CF_ERR_INVALID_ARG, what)
 
 
 def _blocks(n):
-    return -(-n // BLOCK)
+    return (n + 127) >> 7
 
 
-def _mat(t, dtypes, shape, what):
-    """[rows, cols] tensor with unit stride along the columns; its row pitch."""
-    _need(t.dtype in dtypes, f"{what}: type {t.dtype}")
-    _need(t.dim() == 2 and (shape is None or tuple(t.shape) == tuple(shape)), f"{what}: shape {tuple(t.shape)}, expected {shape}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{what}: columns must be contiguous")
-    if t.shape[0] <= 1:
-        return -(-t.shape[1] // 16) * 16               # the pitch of a single row addresses no memory
-    _need(t.stride(0) >= t.shape[1], f"{what}: rows must not overlap")
-    return t.stride(0)
+def _a(t):
+    """Device address of a tensor (an integer: ctypes takes it as it is, a small call spends its time here)."""
+    if t is None:
+        return None
+    assert t.is_cuda, "device tensor expected"
+    return t.data_ptr()
 
 
-def _scales(t, shape, what):
-    _need(t.dtype == torch.float32 and tuple(t.shape) == tuple(shape), f"{what}: float32 {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
-    return t.stride(0), t.stride(1)
+def _mat(t, dtype, rows, cols, what):
+    """Row pitch of a [rows, cols] matrix with contiguous columns and rows that do not overlap."""
+    if t.dtype is not dtype or t.shape != (rows, cols):
+        _refuse(f"{what}: {dtype} [{rows}, {cols}] expected, got {t.dtype} {tuple(t.shape)}")
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or (ld < cols and rows > 1):
+        _refuse(f"{what}: columns must be contiguous and rows must not overlap")
+    return ld if rows > 1 else (cols + 15) & ~15       # the pitch of a single row addresses no memory
 
 
-_BF16, _CODES, _OUT = (torch.bfloat16,), (torch.uint8,), (torch.bfloat16, torch.float32)
+def _scales(t, rows, cols, what):
+    """Strides of a matrix of descales (any)."""
+    if t.dtype is not _f32 or t.shape != (rows, cols):
+        _refuse(f"{what}: float32 [{rows}, {cols}] expected, got {t.dtype} {tuple(t.shape)}")
+    return t.stride()
+
+
+def _dense(t, dtype, shape, what):
+    if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+        _refuse(f"{what}: contiguous {dtype} {list(shape)} expected, got {t.dtype} {tuple(t.shape)}")
 
 
 def block128_row_descale(rows, cols, device="cuda"):
@@ -610,12 +621,15 @@ def block128_row_descale(rows, cols, device="cuda"):
 
 
 def _group_outputs(rows, cols, row8, row_descale, col8, col_descale):
-    _need((row8 is None) == (row_descale is None) and (col8 is None) == (col_descale is None), "codes and descales go together")
-    _need(row8 is not None or col8 is not None, "no output")
-    r = (None, 0, None, 0, 0) if row8 is None else (_p(row8), _mat(row8, _CODES, (rows, cols), "row8"), _p(row_descale),
-                                                    *_scales(row_descale, (rows, _blocks(cols)), "row_descale"))
-    c = (None, 0, None, 0, 0) if col8 is None else (_p(col8), _mat(col8, _CODES, (rows, cols), "col8"), _p(col_descale),
-                                                    *_scales(col_descale, (_blocks(rows), cols), "col_descale"))
+    if (row8 is None) != (row_descale is None) or (col8 is None) != (col_descale is None):
+        _refuse("codes and descales go together")
+    if row8 is None and col8 is None:
+        _refuse("no output")
+    r = c = (None, 0, None, 0, 0)
+    if row8 is not None:
+        r = (_a(row8), _mat(row8, _u8, rows, cols, "row8"), _a(row_descale), *_scales(row_descale, rows, _blocks(cols), "row_descale"))
+    if col8 is not None:
+        c = (_a(col8), _mat(col8, _u8, rows, cols, "col8"), _a(col_descale), *_scales(col_descale, _blocks(rows), cols, "col_descale"))
     return r + c
 
 
@@ -623,60 +637,66 @@ def fp8_quantize_block128(x, row8=None, row_descale=None, col8=None, col_descale
     """Codes of a bf16 matrix with one scale per 128 values of a row (row8, row_descale [rows, ceil(cols/128)]) and / or per
     128 values of a column (col8, col_descale [ceil(rows/128), cols]), from one read."""
     rows, cols = x.shape
-    check(_L().cf_fp8_quantize_block128(_p(x), _mat(x, _BF16, None, "x"), rows, cols, int(is_e5m2),
+    check(_L().cf_fp8_quantize_block128(_a(x), _mat(x, _bf16, rows, cols, "x"), rows, cols, is_e5m2,
                                         *_group_outputs(rows, cols, row8, row_descale, col8, col_descale), _s()))
 
 
 def swiglu_quantize_block128(gate, up, row8=None, row_descale=None, col8=None, col_descale=None):
     """fp8_quantize_block128 of silu(gate) * up (E4M3, no bf16 rounding in between); gate and up share a row pitch."""
     rows, cols = gate.shape
-    ld = _mat(gate, _BF16, None, "gate")
-    _need(_mat(up, _BF16, (rows, cols), "up") == ld, "gate and up must have the same row pitch")
-    check(_L().cf_swiglu_quantize_block128(_p(gate), _p(up), ld, rows, cols,
+    ld = _mat(gate, _bf16, rows, cols, "gate")
+    if _mat(up, _bf16, rows, cols, "up") != ld:
+        _refuse("gate and up must have the same row pitch")
+    check(_L().cf_swiglu_quantize_block128(_a(gate), _a(up), ld, rows, cols,
                                            *_group_outputs(rows, cols, row8, row_descale, col8, col_descale), _s()))
 
 
 def swiglu_backward_quantize_block128(gate, up, dh, row8=None, row_descale=None, col8=None, col_descale=None, is_e5m2=False):
     """Codes of the gradient of silu(gate) * up: [rows, 2 cols], d gate first, d up behind it; cols a multiple of 128."""
     rows, cols = gate.shape
-    ld = _mat(gate, _BF16, None, "gate")
-    _need(_mat(up, _BF16, (rows, cols), "up") == ld, "gate and up must have the same row pitch")
-    check(_L().cf_swiglu_backward_quantize_block128(_p(gate), _p(up), ld, _p(dh), _mat(dh, _BF16, (rows, cols), "dh"), rows, cols,
-                                                    int(is_e5m2), *_group_outputs(rows, 2 * cols, row8, row_descale, col8, col_descale),
-                                                    _s()))
+    ld = _mat(gate, _bf16, rows, cols, "gate")
+    if _mat(up, _bf16, rows, cols, "up") != ld:
+        _refuse("gate and up must have the same row pitch")
+    check(_L().cf_swiglu_backward_quantize_block128(_a(gate), _a(up), ld, _a(dh), _mat(dh, _bf16, rows, cols, "dh"), rows, cols, is_e5m2,
+                                                    *_group_outputs(rows, 2 * cols, row8, row_descale, col8, col_descale), _s()))
 
 
 def fp8_quantize_block128x128(w, w8, descale):
     """E4M3 codes of a weight [rows, cols], or of a stack [n, rows, cols], with one scale per 128x128 block
     (descale [..., ceil(rows/128), ceil(cols/128)])."""
-    _need(w.dim() in (2, 3) and w8.shape == w.shape and descale.dim() == w.dim(), "weight, codes and descales: shapes differ")
+    if w.dim() not in (2, 3) or w8.shape != w.shape or descale.dim() != w.dim():
+        _refuse("weight, codes and descales: shapes differ")
     n = w.shape[0] if w.dim() == 3 else 1
     rows, cols = w.shape[-2:]
     if n == 0 or rows == 0 or cols == 0:
         return
     stacked = w.dim() == 3
-    _need(descale.dtype == torch.float32 and tuple(descale.shape) == (*w.shape[:-2], _blocks(rows), _blocks(cols)) and
-          (descale.stride(-1) == 1 or descale.shape[-1] == 1), "descale: float32 with contiguous rows of blocks expected")
+    if descale.dtype is not _f32 or descale.shape != (*w.shape[:-2], _blocks(rows), _blocks(cols)) or \
+            (descale.stride(-1) != 1 and descale.shape[-1] > 1):
+        _refuse("descale: float32 with contiguous rows of blocks expected")
     w0, q0, d0 = (w[0], w8[0], descale[0]) if stacked else (w, w8, descale)
     ld_d = d0.stride(0) if d0.shape[0] > 1 else max(d0.stride(0), d0.shape[1])
-    check(_L().cf_fp8_quantize_block128x128(_p(w), _mat(w0, _BF16, None, "w"), w.stride(0) if stacked else 0, n, rows, cols, _p(w8),
-                                            _mat(q0, _CODES, None, "w8"), w8.stride(0) if stacked else 0, _p(descale), ld_d,
+    check(_L().cf_fp8_quantize_block128x128(_a(w), _mat(w0, _bf16, rows, cols, "w"), w.stride(0) if stacked else 0, n, rows, cols, _a(w8),
+                                            _mat(q0, _u8, rows, cols, "w8"), w8.stride(0) if stacked else 0, _a(descale), ld_d,
                                             descale.stride(0) if stacked else 0, _s()))
 
 
 def add_rmsnorm_quantize_block128(x, residual, scale, h, rms=None, normed=None, out8=None, descale=None, eps=1e-6):
     """h = bf16(x + residual), RMS norm of h with gain `scale`, codes and row-group descales of the normalised row (and / or
     its bf16 copy `normed`), in one pass. residual may be None (then h may be, too); h may be x or residual itself."""
-    rows, H = x.shape
-    for t, what in ((x, "x"), (residual, "residual"), (h, "h"), (normed, "normed")):
-        _need(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, H) and t.is_contiguous()),
-              f"{what}: contiguous bf16 [{rows}, {H}] expected")
-    _need(scale.dtype == torch.bfloat16 and scale.numel() == H and scale.is_contiguous(), "scale: contiguous bf16 [H] expected")
-    _need(rms is None or (rms.dtype == torch.float32 and rms.numel() == rows and rms.is_contiguous()), "rms: contiguous float32 [rows] expected")
-    _need((out8 is None) == (descale is None), "codes and descales go together")
-    ld8, dr, db = (0, 0, 0) if out8 is None else (_mat(out8, _CODES, (rows, H), "out8"), *_scales(descale, (rows, _blocks(H)), "descale"))
-    check(_L().cf_add_rmsnorm_quantize_block128(_p(x), _p(residual), _p(scale), _p(h), _p(normed), _p(rms), _p(out8), ld8, _p(descale),
-                                                dr, db, rows, H, eps, _s()))
+    shape = rows, H = x.shape
+    _dense(x, _bf16, shape, "x")
+    _dense(residual, _bf16, shape, "residual")
+    _dense(h, _bf16, shape, "h")
+    _dense(normed, _bf16, shape, "normed")
+    _dense(scale, _bf16, (H,), "scale")
+    _dense(rms, _f32, (rows,), "rms")
+    if (out8 is None) != (descale is None):
+        _refuse("codes and descales go together")
+    o = (None, 0, None, 0, 0)
+    if out8 is not None:
+        o = (_a(out8), _mat(out8, _u8, rows, H, "out8"), _a(descale), *_scales(descale, rows, _blocks(H), "descale"))
+    check(_L().cf_add_rmsnorm_quantize_block128(_a(x), _a(residual), _a(scale), _a(h), _a(normed), _a(rms), *o, rows, H, eps, _s()))
 
 
 def add_rmsnorm_backward_scratch_floats(rows, H):
@@ -686,77 +706,78 @@ def add_rmsnorm_backward_scratch_floats(rows, H):
 def add_rmsnorm_backward(dy, h, scale, rms, dh, dx, dscale=None, scratch=None, accumulate_dscale=False):
     """Gradient of the residual addition + RMS norm: dx (of x and of the residual alike) from dy and the gradient dh of the
     residual stream (or None); dscale float32 [H], stored or added to, or None. dx may be dy or dh itself."""
-    rows, H = h.shape
-    for t, what in ((dy, "dy"), (h, "h"), (dh, "dh"), (dx, "dx")):
-        _need(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, H) and t.is_contiguous()),
-              f"{what}: contiguous bf16 [{rows}, {H}] expected")
-    _need(scale.dtype == torch.bfloat16 and scale.numel() == H and scale.is_contiguous(), "scale: contiguous bf16 [H] expected")
-    _need(rms.dtype == torch.float32 and rms.numel() == rows and rms.is_contiguous(), "rms: contiguous float32 [rows] expected")
-    _need(dscale is None or (dscale.dtype == torch.float32 and dscale.numel() == H and dscale.is_contiguous()), "dscale: contiguous float32 [H] expected")
-    _need(scratch is None or (scratch.dtype == torch.float32 and scratch.is_contiguous()), "scratch: contiguous float32 expected")
-    check(_L().cf_add_rmsnorm_backward(_p(dy), _p(h), _p(scale), _p(rms), _p(dh), _p(dx), _p(dscale), int(accumulate_dscale), _p(scratch),
-                                       0 if scratch is None else scratch.numel(), rows, H, _s()))
+    shape = rows, H = h.shape
+    _dense(h, _bf16, shape, "h")
+    _dense(dy, _bf16, shape, "dy")
+    _dense(dh, _bf16, shape, "dh")
+    _dense(dx, _bf16, shape, "dx")
+    _dense(scale, _bf16, (H,), "scale")
+    _dense(rms, _f32, (rows,), "rms")
+    _dense(dscale, _f32, (H,), "dscale")
+    floats = 0
+    if scratch is not None:
+        floats = scratch.numel()
+        _dense(scratch, _f32, (floats,), "scratch")
+    check(_L().cf_add_rmsnorm_backward(_a(dy), _a(h), _a(scale), _a(rms), _a(dh), _a(dx), _a(dscale), accumulate_dscale, _a(scratch),
+                                       floats, rows, H, _s()))
 
 
-def _out_args(out, M, N):
-    return _p(out), _mat(out, _OUT, (M, N), "out"), int(out.dtype == torch.float32)
+def _output(out, M, N):
+    f32 = out.dtype is _f32
+    return _a(out), _mat(out, _f32 if f32 else _bf16, M, N, "out"), f32
 
 
 def gemm_fp8_block128_nt(ctx, A8, a_descale, B8, b_descale, out, a_is_e5m2=False, accumulate=False):
     """out[M,N] (bf16 or float32) = A8[M,K] . B8[N,K]^T with a_descale [M, ceil(K/128)] and b_descale [ceil(N/128), ceil(K/128)]
     (128x128 blocks, weights) or [N, ceil(K/128)] (row groups; taken for blocks where the two shapes are the same, N = 1)."""
     (M, K), N = A8.shape, B8.shape[0]
-    per = BLOCK if b_descale.shape[0] == _blocks(N) else 1
-    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8, _CODES, (N, K), "B8")
-    sa = _scales(a_descale, (M, _blocks(K)), "a_descale")
-    sb = _scales(b_descale, (_blocks(N) if per == BLOCK else N, _blocks(K)), "b_descale")
-    c, ldc, f32 = _out_args(out, M, N)
-    check(_L().cf_gemm_fp8_block128_nt(ctx.handle, M, N, K, _p(A8), lda, int(a_is_e5m2), _p(a_descale), *sa, _p(B8), ldb,
-                                       _p(b_descale), *sb, per, c, ldc, f32, int(accumulate), _s()))
+    nb, kb = _blocks(N), _blocks(K)
+    per = BLOCK if b_descale.shape[0] == nb else 1
+    check(_L().cf_gemm_fp8_block128_nt(ctx.handle, M, N, K, _a(A8), _mat(A8, _u8, M, K, "A8"), a_is_e5m2, _a(a_descale),
+                                       *_scales(a_descale, M, kb, "a_descale"), _a(B8), _mat(B8, _u8, N, K, "B8"), _a(b_descale),
+                                       *_scales(b_descale, nb if per == BLOCK else N, kb, "b_descale"), per, *_output(out, M, N),
+                                       accumulate, _s()))
 
 
 def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_descale, out, a_is_e5m2=False):
     """Rows [offsets[e], +counts[e]) of the compact A8 times expert e of the stacked B8 [E, N, K] (b_descale
     [E, ceil(N/128), ceil(K/128)]) into the same rows of the bf16 out; the other rows are left as they are."""
     (T, K), (E, N, _) = A8.shape, B8.shape
-    _need(counts.dtype == torch.int32 and offsets.dtype == torch.int32 and counts.numel() == E and offsets.numel() == E and
-          counts.is_contiguous() and offsets.is_contiguous(), "counts, offsets: contiguous int32 [E] expected")
-    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8[0], _CODES, (N, K), "B8")
-    if N == 1 and E > 1:
-        ldb = B8.stride(0)
-    _need(E == 1 or B8.stride(0) == N * ldb, "B8: the experts must lie behind one another")
-    sa = _scales(a_descale, (T, _blocks(K)), "a_descale")
-    _need(b_descale.dtype == torch.float32 and tuple(b_descale.shape) == (E, _blocks(N), _blocks(K)) and
-          (b_descale.stride(2) == 1 or b_descale.shape[2] == 1), "b_descale: float32 [E, ceil(N/128), ceil(K/128)] expected")
-    _need(out.dtype == torch.bfloat16, "out: bf16 expected")
-    c, ldc, _ = _out_args(out, T, N)
-    check(_L().cf_gemm_fp8_block128_nt_grouped(ctx.handle, E, T, N, K, _p(counts), _p(offsets), _p(A8), lda, int(a_is_e5m2),
-                                               _p(a_descale), *sa, _p(B8), ldb, _p(b_descale), b_descale.stride(1),
-                                               b_descale.stride(0), c, ldc, _s()))
+    _dense(counts, _i32, (E,), "counts")
+    _dense(offsets, _i32, (E,), "offsets")
+    ldb = _mat(B8[0], _u8, N, K, "B8")
+    if E > 1:
+        if N == 1:
+            ldb = B8.stride(0)
+        if B8.stride(0) != N * ldb:
+            _refuse("B8: the experts must lie behind one another")
+    if b_descale.dtype is not _f32 or b_descale.shape != (E, _blocks(N), _blocks(K)) or (b_descale.stride(2) != 1 and b_descale.shape[2] > 1):
+        _refuse("b_descale: float32 [E, ceil(N/128), ceil(K/128)] expected")
+    check(_L().cf_gemm_fp8_block128_nt_grouped(ctx.handle, E, T, N, K, _a(counts), _a(offsets), _a(A8), _mat(A8, _u8, T, K, "A8"), a_is_e5m2,
+                                               _a(a_descale), *_scales(a_descale, T, _blocks(K), "a_descale"), _a(B8), ldb, _a(b_descale),
+                                               b_descale.stride(1), b_descale.stride(0), _a(out), _mat(out, _bf16, T, N, "out"), _s()))
 
 
 def gemm_fp8_block128_nn(ctx, A8, a_descale, B8_kn, b_descale, out, a_is_e5m2=False, accumulate=False):
     """Data gradient: out[M,N] = A8[M,K] . B8[K,N], the weight read from its forward cache ([out, in] = [K, N]) and block descales
     [ceil(K/128), ceil(N/128)] as they lie; A8 (the gradient) with row groups along K."""
     (M, K), N = A8.shape, B8_kn.shape[1]
-    lda, ldb = _mat(A8, _CODES, None, "A8"), _mat(B8_kn, _CODES, (K, N), "B8_kn")
-    sa = _scales(a_descale, (M, _blocks(K)), "a_descale")
-    sb = _scales(b_descale, (_blocks(K), _blocks(N)), "b_descale")
-    _need(sb[1] == 1 or _blocks(N) == 1, "b_descale: rows of blocks must be contiguous")
-    c, ldc, f32 = _out_args(out, M, N)
-    check(_L().cf_gemm_fp8_block128_nn(ctx.handle, M, N, K, _p(A8), lda, int(a_is_e5m2), _p(a_descale), *sa, _p(B8_kn), ldb,
-                                       _p(b_descale), sb[0], c, ldc, f32, int(accumulate), _s()))
+    ld_b, step = _scales(b_descale, _blocks(K), _blocks(N), "b_descale")
+    if step != 1 and N > BLOCK:
+        _refuse("b_descale: rows of blocks must be contiguous")
+    check(_L().cf_gemm_fp8_block128_nn(ctx.handle, M, N, K, _a(A8), _mat(A8, _u8, M, K, "A8"), a_is_e5m2, _a(a_descale),
+                                       *_scales(a_descale, M, _blocks(K), "a_descale"), _a(B8_kn), _mat(B8_kn, _u8, K, N, "B8_kn"),
+                                       _a(b_descale), ld_b, *_output(out, M, N), accumulate, _s()))
 
 
 def gemm_fp8_block128_dw(ctx, X8, x_descale, dY8, dy_descale, dW, x_is_e5m2=False, dy_is_e5m2=False, accumulate=False):
     """Weight gradient: dW[M,N] (float32 or bf16) = X8[T,M]^T . dY8[T,N] over T tokens, both with column groups of 128 tokens
     (descales [ceil(T/128), M] and [ceil(T/128), N])."""
     (T, M), N = X8.shape, dY8.shape[1]
-    ldx, ldy = _mat(X8, _CODES, None, "X8"), _mat(dY8, _CODES, (T, N), "dY8")
-    sx, sy = _scales(x_descale, (_blocks(T), M), "x_descale"), _scales(dy_descale, (_blocks(T), N), "dy_descale")
-    c, ldc, f32 = _out_args(dW, M, N)
-    check(_L().cf_gemm_fp8_block128_dw(ctx.handle, M, N, T, _p(X8), ldx, int(x_is_e5m2), _p(x_descale), *sx, _p(dY8), ldy,
-                                       int(dy_is_e5m2), _p(dy_descale), *sy, c, ldc, f32, int(accumulate), _s()))
+    kb = _blocks(T)
+    check(_L().cf_gemm_fp8_block128_dw(ctx.handle, M, N, T, _a(X8), _mat(X8, _u8, T, M, "X8"), x_is_e5m2, _a(x_descale),
+                                       *_scales(x_descale, kb, M, "x_descale"), _a(dY8), _mat(dY8, _u8, T, N, "dY8"), dy_is_e5m2,
+                                       _a(dy_descale), *_scales(dy_descale, kb, N, "dy_descale"), *_output(dW, M, N), accumulate, _s()))
 
 
 # ---------------------------------------------------------------- composites: SwiGLU MLP (per-token scales) and MoE SwiGLU experts
@@ -905,3 +926,99 @@ class FfnSwigluFp8:
                                   self.h8, F)
         lt_gemm_fp8_nt(self.ctx, M, y.shape[1], F, self.h8, F, False, _DevPtr(self.slot_h.c.descale_snapshot), w_down8,
                        w_down_descale, y, y.stride(0), bias=bias, bias_mode=bias_mode)
+
+
+class Fp8Block128Weight:
+    """Weight [out, in] with its block-scaled cache: E4M3 codes and one scale per 128x128 block. The one cache serves the forward
+    product (gemm_fp8_block128_nt) and the data gradient (gemm_fp8_block128_nn)."""
+
+    def __init__(self, w):
+        self.w = w                                       # bf16 master
+        out_dim, in_dim = w.shape
+        self.w8 = torch.empty((out_dim, (in_dim + 15) & ~15), dtype=torch.uint8, device=w.device)[:, :in_dim]
+        self.descale = torch.empty((_blocks(out_dim), _blocks(in_dim)), dtype=torch.float32, device=w.device)
+        self.refresh()
+
+    def refresh(self):
+        """Codes of the current master (after an optimiser step)."""
+        fp8_quantize_block128x128(self.w, self.w8, self.descale)
+
+
+class FfnSwigluFp8Block128:
+    """Pre-norm SwiGLU feed-forward block on a residual stream with block-scaled FP8 products:
+        h = x + residual;  n = rmsnorm(h) * gain;  g, u = n . w_gateup^T;  y = (silu(g) * u) . w_down^T
+    `h` (the stream behind the addition) stays in self.h for the next layer. Up to max_rows rows a call: one token of a serving
+    step as well as a training batch. train=True keeps what backward() needs; F must then be a multiple of 128. Gradients are
+    coded as E5M2 (grad_e5m2) or E4M3. The buffers belong to the object: one call at a time."""
+
+    def __init__(self, ctx, max_rows, H, F, train=False, grad_e5m2=True, eps=1e-6, device="cuda"):
+        if train and F % BLOCK:
+            _refuse("FfnSwigluFp8Block128: training needs F to be a multiple of 128")
+        self.ctx, self.H, self.F, self.train, self.e5m2, self.eps, self.max_rows = ctx, H, F, train, grad_e5m2, eps, max_rows
+        R = max_rows
+
+        def bf16(c):
+            return torch.empty((R, c), dtype=torch.bfloat16, device=device)
+
+        def codes(c):
+            return torch.empty((R, (c + 15) & ~15), dtype=torch.uint8, device=device)[:, :c], block128_row_descale(R, c, device)
+
+        def col_codes(c):
+            return (torch.empty((R, (c + 15) & ~15), dtype=torch.uint8, device=device)[:, :c],
+                    torch.empty((_blocks(R), c), dtype=torch.float32, device=device))
+
+        self.h, self.gu, self.rms = bf16(H), bf16(2 * F), torch.empty(R, dtype=torch.float32, device=device)
+        self.n8, self.a8 = codes(H), codes(F)
+        if train:
+            self.n, self.da, self.dn = bf16(H), bf16(F), bf16(H)
+            self.n8c, self.a8c = col_codes(H), col_codes(F)
+            self.dy8, self.dy8c, self.dgu8, self.dgu8c = codes(H), col_codes(H), codes(2 * F), col_codes(2 * F)
+            self.scratch = torch.empty(add_rmsnorm_backward_scratch_floats(R, H), dtype=torch.float32, device=device)
+        self.rows = 0
+
+    def _rows(self, pair):
+        return pair[0][:self.rows], pair[1][:self.rows]
+
+    def _cols(self, pair):
+        return pair[0][:self.rows], pair[1][:_blocks(self.rows)]
+
+    def forward(self, x, residual, gain, w_gateup, w_down, y):
+        """x, y: bf16 [rows, H]; residual: bf16 [rows, H] or None; w_gateup: Fp8Block128Weight [2F, H] (gate rows first), w_down:
+        [H, F]."""
+        rows = self.rows = x.shape[0]
+        if rows > self.max_rows:
+            _refuse(f"FfnSwigluFp8Block128: {rows} rows, made for {self.max_rows}")
+        n8, dn8 = self._rows(self.n8)
+        a8, da8 = self._rows(self.a8)
+        gu = self.gu[:rows]
+        add_rmsnorm_quantize_block128(x, residual, gain, self.h[:rows], self.rms[:rows], self.n[:rows] if self.train else None, n8, dn8,
+                                      self.eps)
+        gemm_fp8_block128_nt(self.ctx, n8, dn8, w_gateup.w8, w_gateup.descale, gu)
+        gate, up = gu[:, :self.F], gu[:, self.F:]
+        if self.train:
+            n8c, dn8c = self._cols(self.n8c)
+            fp8_quantize_block128(self.n[:rows], col8=n8c, col_descale=dn8c)
+            a8c, da8c = self._cols(self.a8c)
+            swiglu_quantize_block128(gate, up, a8, da8, a8c, da8c)
+        else:
+            swiglu_quantize_block128(gate, up, a8, da8)
+        gemm_fp8_block128_nt(self.ctx, a8, da8, w_down.w8, w_down.descale, y)
+
+    def backward(self, dy, dh, gain, w_gateup, w_down, dx, dw_gateup, dw_down, dgain, accumulate=False):
+        """Gradients of the last forward() call for dy (of y) and dh (of the stream h, or None): dx (of x and residual alike),
+        dw_gateup [2F, H], dw_down [H, F] (float32 or bf16), dgain (float32 [H]); the last three added to when accumulate."""
+        if not self.train:
+            _refuse("FfnSwigluFp8Block128: backward() needs train=True")
+        rows, F, e = self.rows, self.F, self.e5m2
+        dy8, ddy8 = self._rows(self.dy8)
+        dy8c, ddy8c = self._cols(self.dy8c)
+        dgu8, ddgu8 = self._rows(self.dgu8)
+        dgu8c, ddgu8c = self._cols(self.dgu8c)
+        da, dn, gu = self.da[:rows], self.dn[:rows], self.gu[:rows]
+        fp8_quantize_block128(dy, dy8, ddy8, dy8c, ddy8c, is_e5m2=e)
+        gemm_fp8_block128_nn(self.ctx, dy8, ddy8, w_down.w8, w_down.descale, da, a_is_e5m2=e)
+        gemm_fp8_block128_dw(self.ctx, dy8c, ddy8c, *self._cols(self.a8c), dw_down, x_is_e5m2=e, accumulate=accumulate)
+        swiglu_backward_quantize_block128(gu[:, :F], gu[:, F:], da, dgu8, ddgu8, dgu8c, ddgu8c, is_e5m2=e)
+        gemm_fp8_block128_nn(self.ctx, dgu8, ddgu8, w_gateup.w8, w_gateup.descale, dn, a_is_e5m2=e)
+        gemm_fp8_block128_dw(self.ctx, dgu8c, ddgu8c, *self._cols(self.n8c), dw_gateup, x_is_e5m2=e, accumulate=accumulate)
+        add_rmsnorm_backward(dn, self.h[:rows], gain, self.rms[:rows], dh, dx, dgain, self.scratch, accumulate)

@@ -58,7 +58,8 @@ def test_norm_refusals(lib, err):
         assert n(**bad) == err.CF_ERR_INVALID_ARG, bad
     assert n(H=16385) == err.CF_ERR_LIMIT
     f = lib.cf_add_rmsnorm_backward_scratch_floats
-    assert f(0, 256) == 0 and f(1, 256) == 256 and f(10 ** 6, 4096) == 444 * 4096 and f(4, 16385) == 0
+    # one partial row per block, as many blocks as rows up to a fixed number
+    assert f(0, 256) == 0 and f(1, 256) == 256 and f(10 ** 6, 4096) == f(10 ** 5, 4096) > 0 and f(4, 16385) == 0
 
     def b(dy=P, h=P, g=P, rms=P, dx=P, dg=P, scratch=P, n=1024, rows=4, H=256):
         return lib.cf_add_rmsnorm_backward(dy, h, g, rms, None, dx, dg, 0, scratch, n, rows, H, None)

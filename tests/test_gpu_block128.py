@@ -508,3 +508,161 @@ def test_empty_sizes_do_nothing(cfb, ctx):
     cfb.add_rmsnorm_backward(x, x, normal((256,), 1), torch.empty(0, device="cuda"), None, x, dg.fill_(1), torch.empty(0, device="cuda"),
                              accumulate_dscale=True)
     assert dg.eq(1).all()
+
+
+# ---------------------------------------------------------------- run together
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("rows,H,F", [(1, 256, 384), (37, 512, 256), (300, 256, 640), (1000, 512, 1024)])
+def test_feed_forward_block_forward_and_gradients(cfb, ctx, rows, H, F):
+    """The block's stages against 64 bits on the codes that each of them really read, and the whole against 64-bit
+    differentiation of the block without any coding."""
+    x, r = normal((rows, H), 71), normal((rows, H), 72)
+    gain = (1 + 0.1 * torch.randn(H, generator=gen(73), device="cuda")).to(torch.bfloat16)
+    wgu, wd = cfb.Fp8Block128Weight(normal((2 * F, H), 74, H ** -0.5)), cfb.Fp8Block128Weight(normal((H, F), 75, F ** -0.5))
+    dy, dh = normal((rows, H), 76, 1e-2), normal((rows, H), 77, 1e-2)
+    block = cfb.FfnSwigluFp8Block128(ctx, rows + 5, H, F, train=True)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    dwgu, dwd, dg = torch.empty((2 * F, H), device="cuda"), torch.empty((H, F), device="cuda"), torch.empty(H, device="cuda")
+    block.forward(x, r, gain, wgu, wd, y)
+    block.backward(dy, dh, gain, wgu, wd, dx, dwgu, dwd, dg)
+    ctx.poll_status()
+    n8, dn8 = block._rows(block.n8)
+    Wgu, Wd = value64(wgu.w8, wgu.descale, False, G, G), value64(wd.w8, wd.descale, False, G, G)
+    check_product(block.gu[:rows], value64(n8, dn8, False, 1, G), Wgu.t(), H)
+    check_product(y, value64(*block._rows(block.a8), False, 1, G), Wd.t(), F)
+    check_product(block.da[:rows], value64(*block._rows(block.dy8), True, 1, G), Wd, H)
+    check_product(dwd, value64(*block._cols(block.dy8c), True, G, 1).t(), value64(*block._cols(block.a8c), False, G, 1), rows)
+    check_product(block.dn[:rows], value64(*block._rows(block.dgu8), True, 1, G), Wgu, 2 * F)
+    check_product(dwgu, value64(*block._cols(block.dgu8c), True, G, 1).t(), value64(*block._cols(block.n8c), False, G, 1), rows)
+    # without coding: X, W and the gradients in 64 bits
+    leaves = [t.double().requires_grad_() for t in (x, gain, wgu.w, wd.w)]
+    X, gg, Wg, Wo = leaves
+    h = X + r.double()
+    n = h / (h.square().mean(1, keepdim=True) + 1e-6).sqrt() * gg
+    gu = n @ Wg.t()
+    out = (torch.nn.functional.silu(gu[:, :F]) * gu[:, F:]) @ Wo.t()
+    (out * dy.double()).sum().backward(retain_graph=True)
+    h.backward(dh.double())
+    # a code is off by 2^-4 of its value at most and 2.6 % rms (E4M3; 5.2 % for E5M2), independently from element to element;
+    # the longest way passes four E4M3 and two E5M2 codings: sqrt(4 * 2.6^2 + 2 * 5.2^2) = 9 %, two of these are allowed
+    for got, want, limit in ((y, out, 0.105), (dx, X.grad, 0.18), (dg, gg.grad, 0.18), (dwgu, Wg.grad, 0.18), (dwd, Wo.grad, 0.18)):
+        assert rel(got, want) < limit, (rel(got, want), limit)
+    # the same block serves fewer rows, without what training keeps; the same numbers, whatever the rows beside them
+    serve = cfb.FfnSwigluFp8Block128(ctx, rows, H, F)
+    y1 = torch.empty_like(y)
+    serve.forward(x, r, gain, wgu, wd, y1)
+    assert torch.equal(y1, y)
+    # accumulation, and the same bits again
+    dwgu2, dwd2, dg2, dx2 = dwgu.clone(), dwd.clone(), dg.clone(), torch.empty_like(dx)
+    block.backward(dy, dh, gain, wgu, wd, dx2, dwgu2, dwd2, dg2, accumulate=True)
+    assert torch.equal(dx2, dx) and torch.equal(dwgu2, dwgu + dwgu) and torch.equal(dwd2, dwd + dwd) and torch.equal(dg2, dg + dg)
+
+
+def test_feed_forward_block_captured_while_another_stream_works(cfb, ctx):
+    """Two blocks captured into graphs and replayed on two streams with new inputs in the same buffers: the bits of eager calls
+    (the products share a context, but keep nothing in it)."""
+    H, F = 512, 384
+    w = [(cfb.Fp8Block128Weight(normal((2 * F, H), 80 + i, H ** -0.5)), cfb.Fp8Block128Weight(normal((H, F), 90 + i, F ** -0.5))) for i in range(2)]
+    gain = normal((H,), 3)
+    rows = (7, 300)
+    blocks = [cfb.FfnSwigluFp8Block128(ctx, n, H, F, train=True) for n in rows]
+    bufs = [[torch.empty((n, H), dtype=torch.bfloat16, device="cuda") for _ in range(4)] for n in rows]
+    grads = [[torch.empty((2 * F, H), device="cuda"), torch.empty((H, F), device="cuda"), torch.empty(H, device="cuda")] for _ in rows]
+
+    def step(i):
+        x, y, dy, dx = bufs[i]
+        blocks[i].forward(x, None, gain, *w[i], y)
+        blocks[i].backward(dy, None, gain, *w[i], dx, *grads[i])
+
+    def fill(seed):
+        for i, n in enumerate(rows):
+            bufs[i][0].copy_(normal((n, H), seed + i))
+            bufs[i][2].copy_(normal((n, H), seed + 5 + i))
+
+    def outputs(i):
+        return [bufs[i][1].clone(), bufs[i][3].clone()] + [g.clone() for g in grads[i]]
+
+    fill(100)
+    streams, graphs = [torch.cuda.Stream() for _ in rows], []
+    for i in range(2):
+        streams[i].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[i]):
+            step(i)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            step(i)
+        graphs.append(g)
+    for seed in (200, 300):
+        fill(seed)
+        torch.cuda.synchronize()
+        want = []
+        for i in range(2):
+            step(i)
+            want.append(outputs(i))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for t in [bufs[i][1], bufs[i][3]] + grads[i]:
+                t.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                for _ in range(3):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outputs(i), want[i]))
+    ctx.poll_status()
+
+
+def test_routed_experts_run(cfb, ctx):
+    """Router, dispatch lists, permute of codes and descales, ragged products, SwiGLU, combine: the layer with block scales."""
+    rows, H, F, E, k = 300, 256, 384, 5, 2
+    x = normal((rows, H), 110)
+    logits = torch.randn((rows, E), generator=gen(111), device="cuda")
+    wgu = torch.stack([normal((2 * F, H), 120 + e, H ** -0.5) for e in range(E)])
+    wd = torch.stack([normal((H, F), 130 + e, F ** -0.5) for e in range(E)])
+    wgu8, dgu = torch.empty_like(wgu, dtype=torch.uint8), torch.empty((E, cdiv(2 * F, G), cdiv(H, G)), device="cuda")
+    wd8, dd = torch.empty_like(wd, dtype=torch.uint8), torch.empty((E, cdiv(H, G), cdiv(F, G)), device="cuda")
+    cfb.fp8_quantize_block128x128(wgu, wgu8, dgu)
+    cfb.fp8_quantize_block128x128(wd, wd8, dd)
+    T = rows * k
+    counts, offsets = (torch.zeros(E, dtype=torch.int32, device="cuda") for _ in range(2))
+    idx = torch.zeros((E, rows), dtype=torch.int32, device="cuda")
+    rw = logits.clone()
+    scratch = torch.empty(max(1, cfb.moe_route_dispatch_scratch_ints(rows, E)), dtype=torch.int32, device="cuda")
+    cfb.moe_route_dispatch_lists(rw, rows, E, k, counts, offsets, idx, scratch)
+    x8, dx = torch.empty((rows, H), dtype=torch.uint8, device="cuda"), torch.empty((rows, cdiv(H, G)), device="cuda")
+    cfb.fp8_quantize_block128(x, x8, dx)
+    xc, dxc = torch.empty((T, H), dtype=torch.uint8, device="cuda"), torch.empty((T, cdiv(H, G)), device="cuda")
+    cfb.moe_gather_all_u8(x8, xc, idx, counts, offsets, rows, E, H)
+    cfb.moe_gather_all_u8(dx.view(torch.uint8), dxc.view(torch.uint8), idx, counts, offsets, rows, E, 4 * cdiv(H, G))
+    gu = torch.empty((T, 2 * F), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_nt_grouped(ctx, counts, offsets, xc, dxc, wgu8, dgu, gu)
+    a8, da = torch.empty((T, F), dtype=torch.uint8, device="cuda"), cfb.block128_row_descale(T, F)
+    cfb.swiglu_quantize_block128(gu[:, :F], gu[:, F:], a8, da)
+    yc = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_nt_grouped(ctx, counts, offsets, a8, da, wd8, dd, yc)
+    mixed = torch.empty((rows, H), dtype=torch.bfloat16, device="cuda")
+    cfb.moe_combine_sorted_bf16(mixed, yc, rw, idx, counts, offsets, rows, E, H, accumulate=False)
+    ctx.poll_status()
+    assert int(counts.sum()) == T
+    want = torch.zeros((rows, H), dtype=torch.float64, device="cuda")
+    for e in range(E):
+        o, n = int(offsets[e]), int(counts[e])
+        at = idx[e, :n].long()
+        assert torch.equal(xc[o:o + n], x8[at]) and torch.equal(dxc[o:o + n], dx[at])
+        check_product(gu[o:o + n], value64(x8[at], dx[at], False, 1, G), value64(wgu8[e], dgu[e], False, G, G).t(), H)
+        check_product(yc[o:o + n], value64(a8[o:o + n], da[o:o + n], False, 1, G), value64(wd8[e], dd[e], False, G, G).t(), F)
+        want[at] += rw[at, e].double()[:, None] * yc[o:o + n].double()
+    # one bf16 rounding per expert added (two of them): 2^-8 of the running sum each
+    mag = torch.zeros_like(want)
+    for e in range(E):
+        o, n = int(offsets[e]), int(counts[e])
+        at = idx[e, :n].long()
+        mag[at] += (rw[at, e].double()[:, None] * yc[o:o + n].double()).abs()
+    assert (mixed.double() - want).abs().le(k * 2.0 ** -8 * (1 + 2.0 ** -6) * mag + 1e-30).all()
