@@ -15,12 +15,14 @@
 // Per block of 128 the MMAs of a CTA need 512 clocks; the promotion needs 64 packed multiply-adds per thread and two warps
 // per scheduler, 128 issue slots, and 128 KB of TMEM reads: it hides behind the MMAs.
 //
-// Narrow form (k_gemm_b128_narrow): few rows of A (tokens). The weights take the MMA's 128-row side and TN tokens its column
+// Narrow form (k_gemm_b128_narrow): few rows of A (tokens), or too few tiles of the wide form to fill the chip. The weights take the MMA's 128-row side and TN tokens its column
 // side, and the contraction is split over a cluster of CTAs whose partial sums meet in distributed shared memory, added in
 // rank order: every weight byte is read once, by enough CTAs to fill the chip, and no atomics are involved.
 //
 // Every wait on an mbarrier is bounded: a wait that gives up raises an abort flag, records a code in the context's status
 // word, drains the CTA's own copies and MMAs, frees TMEM and returns.
+#include <atomic>
+
 #include "cf_common.cuh"
 #include "cf_internal.cuh"
 #include "cf_tc.cuh"
@@ -558,23 +560,58 @@ struct Narrow {
     static constexpr int X_STAGE = TN * BK;
     static constexpr int STAGES = TN <= 32 ? 5 : 4;
     static constexpr int RING = STAGES * (W_STAGE + X_STAGE);
-    static constexpr int SCALES = 4 * 2 * TN * 4;          // per promotion warp two copies of a block's token scales
+    static constexpr int AHEAD = 4;                        // blocks whose scales are on their way
+    // per promotion warp: AHEAD entries of TN token scales and a weight scale per lane, two copies of the products in use
+    static constexpr int WARP_SCALES = AHEAD * (TN + 32) + 2 * TN;
+    static constexpr int SCALES = 4 * WARP_SCALES * 4;
     static constexpr int TMEM = 2 * TN < 32 ? 32 : 2 * TN;
     static constexpr int PARTIAL = TN * 128 * 4;           // overlays the ring after the last block
     static constexpr int SMEM_BYTES = RING + SCALES + 1024 + 256;
     static_assert(PARTIAL <= RING, "partial sums overlay the ring");
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
+// The partial sums part[token][128 features] of the SPLITS CTAs of a cluster, added in rank order and stored. Four features a
+// thread, all ranks' loads of an item in flight at once: one load after the other (250 clocks each out of another SM) took
+// longer than the product itself, 10.4 us instead of 9.5 for 64 x 4096 x 4096 split eight ways.
+template <int SPLITS>
+__device__ __forceinline__ void join_partials(const Params& p, uint32_t part, int tokens, int rank, int m0, int n0, int vec) {
+    uint32_t base[SPLITS];
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) base[r] = SPLITS == 1 ? part : mapa(part, r);
+#pragma unroll 4
+    for (int i = rank * NARROW_THREADS + threadIdx.x; i < tokens * 32; i += SPLITS * NARROW_THREADS) {
+        float4 v[SPLITS];
+#pragma unroll
+        for (int r = 0; r < SPLITS; ++r) v[r] = ld_cluster_f4(base[r] + i * 16);
+#pragma unroll
+        for (int r = 1; r < SPLITS; ++r) {
+            v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w;
+        }
+        const int m = m0 + i / 32, n = n0 + (i % 32) * 4;
+        if (vec && n + 4 <= p.N) {                           // bf16, stored, 8-byte aligned
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + m * p.ldc + n) =
+                make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
+        } else {
+            const float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) store_value(p, m, n + e, f[e]);
+        }
+    }
+}
+
 // map_w: weights [N, K]; map_x: tokens [M, K]. Grid: x = n tile * splits + rank in the cluster, y = token tile.
-template <int TN>
+// BVEC: every weight row has its own scale (folded in per lane); otherwise the tile's 128 rows share one, which is multiplied
+// into the token scales before they are spread.
+template <int TN, bool BVEC>
 __global__ void __launch_bounds__(NARROW_THREADS)
-k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p, int splits, int b_per) {
+k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p, int splits) {
     using C = Narrow<TN>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -624,9 +661,9 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t tmem_base = *s_tmem;
     pdl_wait();
 
-    float acc[TN];
+    uint64_t acc[TN / 2];                  // lane = output feature, pairs of tokens
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < TN / 2; ++j) acc[j] = 0ull;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -672,49 +709,73 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
         // lane = output feature n, TMEM column = token
         const int quarter = warp & 3;
         const int n = n0 + quarter * 32 + lane;
-        const bool n_ok = n < p.N;
-        const float* sw = p.sb + (n_ok ? (n / b_per) * p.sb_row : 0);
-        float* sc = s_scales + (warp - 2) * 2 * TN;
-        constexpr int PER = (TN + 31) / 32;
-        float xs[PER];
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int m = lane + 32 * q;
-            xs[q] = (m < TN && m0 + m < p.M && kb0 < kb1) ? __ldg(p.sa + (m0 + m) * p.sa_row + kb0 * p.sa_blk) : 0.0f;
-        }
-        float w_next = n_ok && kb0 < kb1 ? __ldg(sw + kb0 * p.sb_blk) : 0.0f;
-        bool ok = true;
-        int it = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int buf = it & 1;
-#pragma unroll
-            for (int q = 0; q < PER; ++q)
-                if (lane + 32 * q < TN) sc[buf * TN + lane + 32 * q] = xs[q];
-            __syncwarp();
-            const float w = w_next;
-            if (kb + 1 < kb1) {
-                if (n_ok) w_next = __ldg(sw + (kb + 1) * p.sb_blk);
+        // the tile's one scale, for every lane (each multiplies it into some of the tokens' scales), or the lane's own row's
+        const bool w_ok = !BVEC || n < p.N;
+        const float* sw = p.sb + (w_ok ? (BVEC ? n : n0 / SB) * p.sb_row : 0) + kb0 * p.sb_blk;
+        constexpr int PER = (TN + 31) / 32, ENTRY = TN + 32;
+        float* ring_f = s_scales + (warp - 2) * C::WARP_SCALES;
+        float* sc = ring_f + C::AHEAD * ENTRY;
+        const uint32_t ring = smem_u32(ring_f) + lane * 4;
+        int f_kb = kb0, f_slot = 0;
+        // every lane copies what it will read itself: no barrier between the copy and its use
+        auto fetch = [&]() {
+            if (f_kb < kb1) {
+                const uint32_t dst = ring + f_slot * (ENTRY * 4);
 #pragma unroll
                 for (int q = 0; q < PER; ++q) {
                     const int m = lane + 32 * q;
-                    if (m < TN && m0 + m < p.M) xs[q] = __ldg(p.sa + (m0 + m) * p.sa_row + (kb + 1) * p.sa_blk);
+                    const bool in = m < TN && m0 + m < p.M;
+                    if (m < TN) cp_async4(dst + 128 * q, in ? p.sa + (m0 + m) * p.sa_row + f_kb * p.sa_blk : p.sa, in);
                 }
+                cp_async4(dst + 4 * TN, sw, w_ok);
+                if (w_ok) sw += p.sb_blk;
+                ++f_kb;
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++f_slot == C::AHEAD) f_slot = 0;
+        };
+        for (int i = 0; i < C::AHEAD; ++i) fetch();
+        bool ok = true;
+        int it = 0, slot = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int buf = it & 1;
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::AHEAD - 1) : "memory");
+            const float w = ring_f[slot * ENTRY + TN + lane];
+#pragma unroll
+            for (int q = 0; q < PER; ++q)
+                if (lane + 32 * q < TN) sc[buf * TN + lane + 32 * q] = ring_f[slot * ENTRY + lane + 32 * q] * (BVEC ? 1.0f : w);
+            __syncwarp();
+            if (++slot == C::AHEAD) slot = 0;
+            fetch();
             if (!mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
+            const uint64_t w2 = pack_f2(w, w);
+            constexpr int CH = TN < 32 ? 16 : 32;          // columns per read, the next one on its way while one is folded in
+            uint32_t v[2][32];
+            if (CH == 32) tmem_ld32(taddr, v[0]); else tmem_ld16(taddr, reinterpret_cast<uint32_t(&)[16]>(v[0]));
 #pragma unroll
-            for (int c = 0; c < TN / 16; ++c) {
-                uint32_t v[16];
-                tmem_ld16(taddr + c * 16, v);
+            for (int c = 0; c < TN / CH; ++c) {
                 tmem_ld_wait();
+                if (c + 1 < TN / CH) {
+                    tmem_ld32(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+                } else {                                   // the block is in registers: its buffer goes back
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar + 8 * buf);
+                }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[j]) * w, sc[buf * TN + c * 16 + j], acc[c * 16 + j]);
+                for (int j = 0; j < CH / 4; ++j) {
+                    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(sc + buf * TN + c * CH + 4 * j);
+                    uint64_t x0 = pack_f2(__uint_as_float(v[c & 1][4 * j]), __uint_as_float(v[c & 1][4 * j + 1]));
+                    uint64_t x1 = pack_f2(__uint_as_float(v[c & 1][4 * j + 2]), __uint_as_float(v[c & 1][4 * j + 3]));
+                    if (BVEC) { x0 = mul_f2(x0, w2); x1 = mul_f2(x1, w2); }
+                    acc[(c * CH) / 2 + 2 * j] = fma_f2(x0, s4.x, acc[(c * CH) / 2 + 2 * j]);
+                    acc[(c * CH) / 2 + 2 * j + 1] = fma_f2(x1, s4.y, acc[(c * CH) / 2 + 2 * j + 1]);
+                }
             }
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty_bar + 8 * buf);
         }
+        cp_async_wait_all();
         if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xa00 | 1); }
     }
 
@@ -725,31 +786,23 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM) : "memory");
     }
-    if (splits == 1) {
-        if (warp >= 2) {
-            const int n = n0 + (warp & 3) * 32 + lane;
-#pragma unroll
-            for (int t = 0; t < TN; ++t)
-                if (n < p.N && m0 + t < p.M) store_value(p, m0 + t, n, acc[t]);
-        }
-        return;
-    }
     float* part = reinterpret_cast<float*>(gen);                 // [TN][128]
     if (warp >= 2) {
         const int f = (warp & 3) * 32 + lane;
 #pragma unroll
-        for (int t = 0; t < TN; ++t) part[t * 128 + f] = acc[t];
+        for (int t = 0; t < TN; t += 2) unpack_f2(acc[t / 2], part[t * 128 + f], part[(t + 1) * 128 + f]);
+    }
+    const int tokens = min(TN, p.M - m0);
+    const int vec = p.out_kind == OUT_BF16 && p.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(p.C) % 8 == 0;
+    if (splits == 1) {
+        __syncthreads();
+        join_partials<1>(p, base, tokens, 0, m0, n0, vec);
+        return;
     }
     cluster_sync_all();
-    if (warp >= 2) {
-        // this CTA adds up the tokens rank, rank + splits, ...: partial sums in rank order
-        const int f = (warp & 3) * 32 + lane;
-        for (int t = rank; t < TN && m0 + t < p.M; t += splits) {
-            float v = 0.0f;
-            for (int r = 0; r < splits; ++r) v += ld_cluster_f32(mapa(base + (t * 128 + f) * 4, r));
-            if (n0 + f < p.N) store_value(p, m0 + t, n0 + f, v);
-        }
-    }
+    if (splits == 2) join_partials<2>(p, base, tokens, rank, m0, n0, vec);
+    else if (splits == 4) join_partials<4>(p, base, tokens, rank, m0, n0, vec);
+    else join_partials<8>(p, base, tokens, rank, m0, n0, vec);
     cluster_sync_all();                                          // the others have read this CTA's sums
 }
 
@@ -808,15 +861,16 @@ int resident_pairs(int* pairs) {
     return CF_OK;
 }
 
-template <int TN>
-int launch_narrow(const CUtensorMap& map_w, const CUtensorMap& map_x, const Params& p, int splits, int b_per, cudaStream_t st) {
+template <int TN, bool BVEC>
+int launch_narrow(const CUtensorMap& map_w, const CUtensorMap& map_x, const Params& p, int splits, cudaStream_t st) {
     using C = Narrow<TN>;
-    static std::once_flag once[64];
+    static std::atomic<int> ready[64];      // the attribute is set once per device (any thread may do it)
     int dev = 0;
     CF_CUDA(cudaGetDevice(&dev));
-    cudaError_t e = cudaSuccess;
-    std::call_once(once[dev & 63], [&] { e = cudaFuncSetAttribute(k_gemm_b128_narrow<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES); });
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(k_gemm_b128_narrow)");
+    if (!ready[dev & 63].load(std::memory_order_acquire)) {
+        CF_CUDA(cudaFuncSetAttribute(k_gemm_b128_narrow<TN, BVEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+        ready[dev & 63].store(1, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(cdiv(p.N, 128) * splits), static_cast<unsigned>(cdiv(p.M, TN)));
     cfg.blockDim = dim3(NARROW_THREADS);
@@ -829,9 +883,13 @@ int launch_narrow(const CUtensorMap& map_w, const CUtensorMap& map_x, const Para
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128_narrow<TN>, map_w, map_x, p, splits, b_per));
+    CF_CUDA(cudaLaunchKernelEx(&cfg, k_gemm_b128_narrow<TN, BVEC>, map_w, map_x, p, splits));
     CF_LAUNCH_CHECK("gemm_b128_narrow");
     return CF_OK;
+}
+template <int TN>
+int launch_narrow_any(const CUtensorMap& map_w, const CUtensorMap& map_x, const Params& p, int splits, int b_per, cudaStream_t st) {
+    return b_per == 1 ? launch_narrow<TN, true>(map_w, map_x, p, splits, st) : launch_narrow<TN, false>(map_w, map_x, p, splits, st);
 }
 
 // a_rows_mem / b_rows_mem: row extents of the two byte matrices in memory. b_per: columns of C per B scale (128 or 1).
@@ -844,26 +902,33 @@ int launch_b128(const char* fn, const void* A, long long lda, const void* B, lon
     int rc = require_sm100();
     if (rc != CF_OK) return rc;
     CUtensorMap map_a, map_b, map_c;
-    // Few rows of a K-major product: the narrow form
-    if (p.groups == 0 && !p.a_mn && !p.b_mn && p.M <= 128) {
-        const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
-        const long long ctas = cdiv(p.N, 128) * cdiv(p.M, tn);
-        const int k_iters = static_cast<int>(cdiv(p.K, BK));
-        int splits = 1;
-        while (splits < 8 && ctas * splits * 2 <= 2ll * sm_count() && k_iters >= 4 * splits) splits *= 2;
-        rc = make_map(&map_b, B, b_rows_mem, p.K, ldb, 128);
-        if (rc == CF_OK) rc = make_map(&map_a, A, p.M, p.K, lda, tn);
-        if (rc != CF_OK) return rc;
-        if (tn == 16) return launch_narrow<16>(map_b, map_a, p, splits, b_per, st);
-        if (tn == 32) return launch_narrow<32>(map_b, map_a, p, splits, b_per, st);
-        if (tn == 64) return launch_narrow<64>(map_b, map_a, p, splits, b_per, st);
-        return launch_narrow<128>(map_b, map_a, p, splits, b_per, st);
-    }
     int pairs = 0;
     rc = resident_pairs(&pairs);
     if (rc != CF_OK) return rc;
     const long long rows_per_group = p.groups > 0 ? p.M / p.groups : p.M;
     const bool pair = p.a_mn || p.b_mn || rows_per_group >= 512;
+    const int k_iters = static_cast<int>(cdiv(p.K, BK));
+    if (p.groups == 0 && !p.a_mn && !p.b_mn) {
+        // The narrow form where it is expected to end first. Its CTAs (two on an SM) take about 0.70 us per block of K, the wide
+        // form's tiles 0.47 (one CTA) or 0.55 (pair); up to 64 rows it reads every weight once and runs at the memory's rate.
+        // Narrow / wide us, N x K: 28672 x 4096: M = 32 21.7 / 25.4, 64 24.3 / 25.6, 96 45 / 26; 4096 x 14336: 64 16.7 / 56,
+        // 256 42 / 56, 384 77 / 56; 4096 x 4096: 128 10.9 / 19.6, 256 15.5 / 19.8, 384 24 / 20; 1024 x 4096: 512 10.9 / 21.
+        const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
+        const long long ctas = cdiv(p.N, 128) * cdiv(p.M, tn), room = 2ll * sm_count();
+        int splits = 1;
+        while (splits < 8 && ctas * splits * 2 <= room && k_iters >= 4 * splits) splits *= 2;
+        const long long wide_tiles = cdiv(p.M, pair ? 256 : 128) * cdiv(p.N, BN);
+        const long long narrow_cost = cdiv(ctas * splits, room) * cdiv(k_iters, splits) * 70;
+        const long long wide_cost = cdiv(wide_tiles, pair ? pairs : sm_count()) * k_iters * (pair ? 55 : 47);
+        if (p.M <= 64 || narrow_cost < wide_cost) {
+            rc = make_map(&map_b, B, b_rows_mem, p.K, ldb, 128);
+            if (rc == CF_OK) rc = make_map(&map_a, A, p.M, p.K, lda, tn);
+            if (rc != CF_OK) return rc;
+            if (tn == 16) return launch_narrow_any<16>(map_b, map_a, p, splits, b_per, st);
+            if (tn == 32) return launch_narrow_any<32>(map_b, map_a, p, splits, b_per, st);
+            return launch_narrow_any<64>(map_b, map_a, p, splits, b_per, st);
+        }
+    }
     rc = p.a_mn ? make_map(&map_a, A, p.K, p.M, lda, BK) : make_map(&map_a, A, p.M, p.K, lda, BM);
     if (rc == CF_OK) rc = p.b_mn ? make_map(&map_b, B, b_rows_mem, p.N, ldb, BK) : make_map(&map_b, B, b_rows_mem, p.K, ldb, pair ? 128 : 256);
     if (rc != CF_OK) return rc;

@@ -513,8 +513,8 @@ int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_sca
  * A8 [M, K] E4M3 or E5M2, row pitch lda; B8 [N, K] E4M3, row pitch ldb; both 16-byte aligned with pitches that are multiples
  * of 16 (CF_ERR_UNSUPPORTED otherwise), K any number. b_rows_per_scale: 128 (weights: db of row n at
  * d[(n / 128) * ld_row + b * ld_block]) or 1 (row groups). C: bf16 or (out_fp32) float, pitch ldc, stored or (accumulate)
- * added to. No float atomics: results do not depend on timing. Up to 128 rows of A take a form that reads every weight
- * once, with the contraction split over a cluster. */
+ * added to. No float atomics: results do not depend on timing. Few rows of A (and products with few tiles) take a form
+ * that reads every weight once per 64 rows, with the contraction split over a cluster; the sums' order then differs. */
 int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
                             long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb, const float* d_b_descale,
                             long long b_descale_ld_row, long long b_descale_ld_block, int b_rows_per_scale, void* d_C, int ldc,
