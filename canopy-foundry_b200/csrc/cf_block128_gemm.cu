@@ -453,10 +453,16 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        uint64_t x = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
-                        if (BVEC) x = mul_f2(x, *reinterpret_cast<const uint64_t*>(cs + c * 32 + 2 * j));
-                        acc[c * 16 + j] = fma_f2(x, s2, acc[c * 16 + j]);
+                    for (int j = 0; j < 16; j += 2) {
+                        uint64_t x0 = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
+                        uint64_t x1 = pack_f2(__uint_as_float(v[c & 1][2 * j + 2]), __uint_as_float(v[c & 1][2 * j + 3]));
+                        if (BVEC) {
+                            const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(cs + c * 32 + 2 * j);
+                            x0 = mul_f2(x0, b4.x);
+                            x1 = mul_f2(x1, b4.y);
+                        }
+                        acc[c * 16 + j] = fma_f2(x0, s2, acc[c * 16 + j]);
+                        acc[c * 16 + j + 1] = fma_f2(x1, s2, acc[c * 16 + j + 1]);
                     }
                 }
                 if (!ok) break;
@@ -905,22 +911,27 @@ int launch_b128(const char* fn, const void* A, long long lda, const void* B, lon
     int pairs = 0;
     rc = resident_pairs(&pairs);
     if (rc != CF_OK) return rc;
-    const long long rows_per_group = p.groups > 0 ? p.M / p.groups : p.M;
-    const bool pair = p.a_mn || p.b_mn || rows_per_group >= 512;
     const int k_iters = static_cast<int>(cdiv(p.K, BK));
+    // CTA pairs or single CTAs: whichever is expected to end first. A block of K takes a pair's tile about 0.55 us, a single CTA's
+    // (half of it) 0.58 with the chip full and 0.47 with less: the promotion sets the pace of both, so what decides is how the
+    // tiles fill the last round. Ragged groups end in half a row block each on average. Measured pair / single: eight ragged
+    // experts, 4096 rows x 4096 x 14336: 331 / 272 us; 1531 x 4104 x 5416: 48 / 60; 8192^3: 522 / 560.
+    const int sms = sm_count();
+    auto tile_count = [&](int tm) { return (p.groups > 0 ? p.M / tm + (p.groups + 1) / 2 : cdiv(p.M, tm)) * cdiv(p.N, BN); };
+    const long long singles = tile_count(128);
+    const long long pair_cost = cdiv(tile_count(256), pairs) * 55, single_cost = cdiv(singles, sms) * (singles <= sms ? 47 : 58);
+    const bool pair = p.a_mn || p.b_mn || pair_cost <= single_cost;
     if (p.groups == 0 && !p.a_mn && !p.b_mn) {
-        // The narrow form where it is expected to end first. Its CTAs (two on an SM) take about 0.70 us per block of K, the wide
-        // form's tiles 0.47 (one CTA) or 0.55 (pair); up to 64 rows it reads every weight once and runs at the memory's rate.
+        // The narrow form where it is expected to end before either. Its CTAs (two on an SM) take about 0.70 us per block of K; up
+        // to 64 rows it reads every weight once and runs at the memory's rate.
         // Narrow / wide us, N x K: 28672 x 4096: M = 32 21.7 / 25.4, 64 24.3 / 25.6, 96 45 / 26; 4096 x 14336: 64 16.7 / 56,
         // 256 42 / 56, 384 77 / 56; 4096 x 4096: 128 10.9 / 19.6, 256 15.5 / 19.8, 384 24 / 20; 1024 x 4096: 512 10.9 / 21.
         const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
-        const long long ctas = cdiv(p.N, 128) * cdiv(p.M, tn), room = 2ll * sm_count();
+        const long long ctas = cdiv(p.N, 128) * cdiv(p.M, tn), room = 2ll * sms;
         int splits = 1;
         while (splits < 8 && ctas * splits * 2 <= room && k_iters >= 4 * splits) splits *= 2;
-        const long long wide_tiles = cdiv(p.M, pair ? 256 : 128) * cdiv(p.N, BN);
         const long long narrow_cost = cdiv(ctas * splits, room) * cdiv(k_iters, splits) * 70;
-        const long long wide_cost = cdiv(wide_tiles, pair ? pairs : sm_count()) * k_iters * (pair ? 55 : 47);
-        if (p.M <= 64 || narrow_cost < wide_cost) {
+        if (p.M <= 64 || narrow_cost < (pair ? pair_cost : single_cost) * k_iters) {
             rc = make_map(&map_b, B, b_rows_mem, p.K, ldb, 128);
             if (rc == CF_OK) rc = make_map(&map_a, A, p.M, p.K, lda, tn);
             if (rc != CF_OK) return rc;
