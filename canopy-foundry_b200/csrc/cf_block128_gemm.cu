@@ -46,13 +46,12 @@ constexpr int kLaunchRegs = 168, kLeanRegs = 56, kWideRegs = 224;
 static_assert(kLeanRegs * 128 + kWideRegs * 256 <= kLaunchRegs * NUM_THREADS, "register shares");
 constexpr int TMEM_COLS = 512;          // two 128x256 fp32 block sums per CTA
 constexpr int C_STAGING = EPI_WARPS * C_BOX_BYTES;
-// Scales on their way from global memory: a ring of blocks, each with the 128 row scales and the column scales (256, or one
-// per 128 columns) of the CTA's tile, filled by a warp of its own with 4-byte asynchronous copies several blocks ahead. A
-// scale's first use misses L1 and often L2 (another line for every block of K): loaded by the promotion warps one block
-// ahead, or copied by them several blocks ahead, the scales took more of their time than the promotion itself.
-constexpr int SCALE_DEPTH = 8;
+// Scales on their way from global memory: per stage of the operand ring the 128 row scales and the column scales (256, or one per
+// 128 columns) of the block, filled by a warp of its own with 4-byte asynchronous copies as soon as the promotion has read the
+// block that had the slot before. They land on the barrier that tells the block's sums are there, so the promotion waits once
+// per block. A scale's first use misses L1 and often L2 (another line for every block of K): loaded by the promotion warps one
+// block ahead, or copied by them several blocks ahead, the scales took more of their time than the promotion itself.
 constexpr int SCALE_ENTRY = BM + BN;                       // floats
-constexpr int SCALE_RING = SCALE_DEPTH * SCALE_ENTRY * 4;
 
 template <bool PAIR>
 struct Cfg {
@@ -62,6 +61,7 @@ struct Cfg {
     static constexpr int B_STAGE = B_ROWS * BK;
     static constexpr int TILE_M = PAIR ? 256 : 128;
     static constexpr int RING = STAGES * (A_STAGE + B_STAGE);
+    static constexpr int SCALE_RING = STAGES * SCALE_ENTRY * 4;
     static constexpr int SMEM_BYTES = RING + C_STAGING + SCALE_RING + 1024 /*alignment slack*/ + 512 /*barriers*/;
 };
 
@@ -213,12 +213,12 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const uint32_t smem_a = base;
     const uint32_t smem_b = base + STAGES * A_STAGE;
     const uint32_t smem_c = smem_b + STAGES * B_STAGE;
-    const uint32_t bars = smem_c + C_STAGING + SCALE_RING;
-    const uint32_t full_bar = bars, done_bar = bars + 8 * STAGES;      // per stage: operands there / block multiplied
-    const uint32_t tempty_bar = bars + 16 * STAGES, drain_bar = tempty_bar + 16;
-    const uint32_t sfull_bar = drain_bar + 16, sempty_bar = sfull_bar + 8 * SCALE_DEPTH;
+    const uint32_t bars = smem_c + C_STAGING + C::SCALE_RING;
+    // per stage: operands there; block multiplied and its scales there; scales read
+    const uint32_t full_bar = bars, done_bar = bars + 8 * STAGES, sempty_bar = bars + 16 * STAGES;
+    const uint32_t tempty_bar = bars + 24 * STAGES, drain_bar = tempty_bar + 16;
     uint8_t* gen = smem_raw + (base - raw);
-    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C_STAGING + SCALE_RING + 16 * STAGES + 48 + 16 * SCALE_DEPTH);
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::RING + C_STAGING + C::SCALE_RING + 24 * STAGES + 32);
     const uint32_t ring = smem_c + C_STAGING;
     const float* ring_f = reinterpret_cast<const float*>(gen + C::RING + C_STAGING);
     volatile int* s_abort = reinterpret_cast<volatile int*>(const_cast<uint32_t*>(s_tmem) + 1);
@@ -232,15 +232,12 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar + 8 * s, 1);
-            mbar_init(done_bar + 8 * s, 1);
+            mbar_init(done_bar + 8 * s, 1 + 32);             // the commit, and the lanes of the scale warp as their copies land
+            mbar_init(sempty_bar + 8 * s, EPI_WARPS);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tempty_bar + 8 * a, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
             mbar_init(drain_bar + 8 * a, 1);
-        }
-        for (int e = 0; e < SCALE_DEPTH; ++e) {
-            mbar_init(sfull_bar + 8 * e, 32);                // the lanes of the scale warp, each when its copies have landed
-            mbar_init(sempty_bar + 8 * e, EPI_WARPS);
         }
         s_abort[0] = 0;
         s_abort[1] = 0;                                      // stays 0: abort source for the drain waits
@@ -387,10 +384,10 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     const bool in = tc_.n0 + lane * SB < p.N;
                     cp_async4(dst + 4 * BM, in ? sb : p.sb, in);
                 }
-                cp_async_arrive(sfull_bar + 8 * e);
+                cp_async_arrive(done_bar + 8 * e);
                 sa += p.sa_blk;
                 sb += p.sb_blk;
-                if (++e == SCALE_DEPTH) { e = 0; phase ^= 1u; }
+                if (++e == STAGES) { e = 0; phase ^= 1u; }
             }
         }
         if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xb00 | 1); }
@@ -405,8 +402,8 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const uint32_t box = smem_c + static_cast<uint32_t>(warp - 4) * C_BOX_BYTES;
         float* box_f = reinterpret_cast<float*>(gen + C::RING + (warp - 4) * C_BOX_BYTES);
         const uint64_t store_policy = l2_policy_evict_first();
-        int it = 0, e = 0, st = 0;                         // block, slot of its scales, its stage
-        uint32_t s_phase = 0, d_phase = 0;
+        int it = 0, st = 0;                                // block, its stage
+        uint32_t d_phase = 0;
         bool ok = true;
         for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
             const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
@@ -419,17 +416,17 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // is folded in, the next one is on its way. A buffer goes back as soon as its last chunk is in registers.
             const uint32_t tcol = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
             uint32_t v[2][32];
-            ok = mbar_wait(sfull_bar + 8 * e, s_phase, s_abort) && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
+            ok = mbar_wait(done_bar + 8 * st, d_phase, s_abort);
             if (!ok) break;
             tcgen05_fence_after();
             tmem_ld32(tcol + (it & 1) * BN, v[0]);
             for (int kb = 0; kb < k_iters; ++kb) {
                 const int buf = it & 1;
-                const float* entry = ring_f + e * SCALE_ENTRY;
+                const float* entry = ring_f + st * SCALE_ENTRY;
                 const float* cs = entry + BM + half * 128;
                 const float s_row = BVEC ? entry[quarter * 32 + lane] : entry[quarter * 32 + lane] * entry[BM + half];
                 const uint64_t s2 = pack_f2(s_row, s_row);
-                const uint32_t done = sempty_bar + 8 * e;
+                const uint32_t done = sempty_bar + 8 * st;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     tmem_ld_wait();
@@ -443,10 +440,9 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             if (!BVEC) mbar_arrive(done);
                         }
                         ++it;
-                        if (++e == SCALE_DEPTH) { e = 0; s_phase ^= 1u; }
                         if (++st == STAGES) { st = 0; d_phase ^= 1u; }
                         if (kb + 1 < k_iters) {
-                            ok = mbar_wait(sfull_bar + 8 * e, s_phase, s_abort) && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
+                            ok = mbar_wait(done_bar + 8 * st, d_phase, s_abort);
                             if (!ok) break;
                             tcgen05_fence_after();
                             tmem_ld32(tcol + (it & 1) * BN, v[0]);
