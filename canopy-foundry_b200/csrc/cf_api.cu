@@ -82,6 +82,7 @@ constexpr int kMaxSlots = 4096;
 constexpr int kHistoryLen = 8;         // kActHistoryLen, src/trainer.cu:3213
 
 int* ctx_status(cf_ctx* c) { return reinterpret_cast<Ctx*>(c)->d_status; }
+int ctx_device(cf_ctx* c) { return reinterpret_cast<Ctx*>(c)->device; }
 void* ctx_workspace(cf_ctx* c, size_t* bytes) {
     Ctx* x = reinterpret_cast<Ctx*>(c);
     *bytes = x->workspace_bytes;

@@ -30,6 +30,7 @@
 namespace cf {
 
 int* ctx_status(cf_ctx* c);
+int ctx_device(cf_ctx* c);
 
 namespace {
 
@@ -895,7 +896,7 @@ int launch_narrow_any(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
 }
 
 // a_rows_mem / b_rows_mem: row extents of the two byte matrices in memory. b_per: columns of C per B scale (128 or 1).
-int launch_b128(const char* fn, const void* A, long long lda, const void* B, long long ldb, long long b_rows_mem, Params p, int b_per,
+int launch_b128(const char* fn, cf_ctx* ctx, const void* A, long long lda, const void* B, long long ldb, long long b_rows_mem, Params p, int b_per,
                 cudaStream_t st) {
     if (!aligned(A, 16) || !aligned(B, 16) || lda % 16 != 0 || ldb % 16 != 0) {
         set_error("%s: the FP8 operands need 16-byte aligned bases and row pitches", fn);
@@ -903,6 +904,10 @@ int launch_b128(const char* fn, const void* A, long long lda, const void* B, lon
     }
     int rc = require_sm100();
     if (rc != CF_OK) return rc;
+    int dev = 0;
+    CF_CUDA(cudaGetDevice(&dev));
+    CF_REQUIRE(dev == ctx_device(ctx), "%s: the context belongs to device %d, the current device is %d", fn, ctx_device(ctx), dev);
+    p.d_status = ctx_status(ctx);
     CUtensorMap map_a, map_b, map_c;
     int pairs = 0;
     rc = resident_pairs(&pairs);
@@ -986,11 +991,21 @@ int check_common(const char* fn, cf_ctx* ctx, int M, int N, int K, const void* A
     CF_REQUIRE(ctx != nullptr, "%s: null context", fn);
     CF_REQUIRE(M >= 0 && N >= 0 && K >= 0, "%s: negative shape", fn);
     if (M == 0 || N == 0) return CF_OK;
-    CF_REQUIRE(K > 0, "%s: an empty contraction is not supported", fn);
-    CF_REQUIRE(A && B && C, "%s: null matrix pointer", fn);
-    CF_REQUIRE(sa && sb, "%s: null descale pointer", fn);
+    constexpr int kMost = 0x7ffffc00;       // tile coordinates are 32-bit
+    if (M > kMost || N > kMost || K > kMost) { set_error("%s: a size beyond 2^31 - 1024", fn); return CF_ERR_LIMIT; }
+    CF_REQUIRE(C, "%s: null output", fn);
     CF_REQUIRE(ldc >= N, "%s: output pitch smaller than a row", fn);
-    CF_REQUIRE(aligned(sa, 4) && aligned(sb, 4) && aligned(C, fp32 ? 4 : 2), "%s: misaligned pointer", fn);
+    CF_REQUIRE(aligned(C, fp32 ? 4 : 2), "%s: misaligned pointer", fn);
+    if (K == 0) return CF_OK;
+    CF_REQUIRE(A && B, "%s: null matrix pointer", fn);
+    CF_REQUIRE(sa && sb, "%s: null descale pointer", fn);
+    CF_REQUIRE(aligned(sa, 4) && aligned(sb, 4), "%s: misaligned pointer", fn);
+    return CF_OK;
+}
+// A sum over nothing (K = 0): zero, or what was there.
+int empty_contraction(void* C, long long ldc, int M, int N, int fp32, int accumulate, cudaStream_t st) {
+    const size_t es = fp32 ? 4 : 2;
+    if (!accumulate) CF_CUDA(cudaMemset2DAsync(C, ldc * es, 0, N * es, M, st));
     return CF_OK;
 }
 
@@ -1008,6 +1023,7 @@ int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
     const char* fn = "cf_gemm_fp8_block128_nt";
     const int rc = check_common(fn, ctx, M, N, K, d_A, d_a_descale, d_B, d_b_descale, d_C, ldc, out_fp32);
     if (rc != CF_OK || M == 0 || N == 0) return rc;
+    if (K == 0) return empty_contraction(d_C, ldc, M, N, out_fp32, accumulate, as_stream(stream));
     CF_REQUIRE(lda >= K && ldb >= K, "%s: operand pitch smaller than a row", fn);
     CF_REQUIRE(b_rows_per_scale == 128 || b_rows_per_scale == 1, "%s: a scale of B covers 128 rows or 1", fn);
     Params p;
@@ -1016,8 +1032,7 @@ int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
     p.sb = d_b_descale; p.sb_row = b_descale_ld_row; p.sb_blk = b_descale_ld_block;
     p.C = d_C; p.ldc = ldc; p.out_kind = out_kind(out_fp32, accumulate);
     p.a_e5m2 = a_is_e5m2 ? 1 : 0;
-    p.d_status = ctx_status(ctx);
-    return launch_b128(fn, d_A, lda, d_B, ldb, N, p, b_rows_per_scale, as_stream(stream));
+    return launch_b128(fn, ctx, d_A, lda, d_B, ldb, N, p, b_rows_per_scale, as_stream(stream));
 }
 
 int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_rows, int N, int K, const int* d_counts,
@@ -1028,7 +1043,9 @@ int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_
     const char* fn = "cf_gemm_fp8_block128_nt_grouped";
     const int rc = check_common(fn, ctx, max_total_rows, N, K, d_A, d_a_descale, d_B, d_b_descale, d_C, ldc, 0);
     if (rc != CF_OK || max_total_rows == 0 || N == 0) return rc;
+    CF_REQUIRE(K > 0, "%s: empty contraction", fn);
     CF_REQUIRE(num_experts > 0 && d_counts && d_offsets, "%s: no groups", fn);
+    if (num_experts > 65536) { set_error("%s: more than 65536 experts", fn); return CF_ERR_LIMIT; }
     CF_REQUIRE(aligned(d_counts, 4) && aligned(d_offsets, 4), "%s: misaligned pointer", fn);
     CF_REQUIRE(lda >= K && ldb >= K, "%s: operand pitch smaller than a row", fn);
     if (static_cast<long long>(num_experts) * N > 0x7fffffffll) { set_error("%s: more than 2^31 weight rows", fn); return CF_ERR_LIMIT; }
@@ -1039,8 +1056,7 @@ int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_
     p.sb = d_b_descale; p.sb_row = b_descale_ld_row; p.sb_blk = 1; p.sb_group = b_descale_stride;
     p.C = d_C; p.ldc = ldc; p.out_kind = OUT_BF16;
     p.a_e5m2 = a_is_e5m2 ? 1 : 0;
-    p.d_status = ctx_status(ctx);
-    return launch_b128(fn, d_A, lda, d_B, ldb, static_cast<long long>(num_experts) * N, p, 128, as_stream(stream));
+    return launch_b128(fn, ctx, d_A, lda, d_B, ldb, static_cast<long long>(num_experts) * N, p, 128, as_stream(stream));
 }
 
 int cf_gemm_fp8_block128_nn(cf_ctx* ctx, int M, int N, int K, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
@@ -1050,6 +1066,7 @@ int cf_gemm_fp8_block128_nn(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
     const char* fn = "cf_gemm_fp8_block128_nn";
     const int rc = check_common(fn, ctx, M, N, K, d_A, d_a_descale, d_B_kn, d_b_descale, d_C, ldc, out_fp32);
     if (rc != CF_OK || M == 0 || N == 0) return rc;
+    if (K == 0) return empty_contraction(d_C, ldc, M, N, out_fp32, accumulate, as_stream(stream));
     CF_REQUIRE(lda >= K && ldb >= N, "%s: operand pitch smaller than a row", fn);
     Params p;
     p.M = M; p.N = N; p.K = K;
@@ -1058,8 +1075,7 @@ int cf_gemm_fp8_block128_nn(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
     p.C = d_C; p.ldc = ldc; p.out_kind = out_kind(out_fp32, accumulate);
     p.a_e5m2 = a_is_e5m2 ? 1 : 0;
     p.b_mn = 1;
-    p.d_status = ctx_status(ctx);
-    return launch_b128(fn, d_A, lda, d_B_kn, ldb, K, p, 128, as_stream(stream));
+    return launch_b128(fn, ctx, d_A, lda, d_B_kn, ldb, K, p, 128, as_stream(stream));
 }
 
 int cf_gemm_fp8_block128_dw(cf_ctx* ctx, int M, int N, int K, const void* d_X, int ldx, int x_is_e5m2, const float* d_x_descale,
@@ -1069,6 +1085,7 @@ int cf_gemm_fp8_block128_dw(cf_ctx* ctx, int M, int N, int K, const void* d_X, i
     const char* fn = "cf_gemm_fp8_block128_dw";
     const int rc = check_common(fn, ctx, M, N, K, d_X, d_x_descale, d_dY, d_dy_descale, d_dW, ldc, out_fp32);
     if (rc != CF_OK || M == 0 || N == 0) return rc;
+    if (K == 0) return empty_contraction(d_dW, ldc, M, N, out_fp32, accumulate, as_stream(stream));
     CF_REQUIRE(ldx >= M && ldy >= N, "%s: operand pitch smaller than a row", fn);
     Params p;
     p.M = M; p.N = N; p.K = K;
@@ -1078,8 +1095,7 @@ int cf_gemm_fp8_block128_dw(cf_ctx* ctx, int M, int N, int K, const void* d_X, i
     p.a_e5m2 = x_is_e5m2 ? 1 : 0;
     p.b_e5m2 = dy_is_e5m2 ? 1 : 0;
     p.a_mn = p.b_mn = 1;
-    p.d_status = ctx_status(ctx);
-    return launch_b128(fn, d_X, ldx, d_dY, ldy, K, p, 1, as_stream(stream));
+    return launch_b128(fn, ctx, d_X, ldx, d_dY, ldy, K, p, 1, as_stream(stream));
 }
 
 }  // extern "C"

@@ -585,12 +585,17 @@ def _blocks(n):
     return (n + 127) >> 7
 
 
+def _on(*tensors):
+    """Every tensor is on the current device, whose stream the call goes to."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _refuse(f"tensors on the current device (cuda:{dev}) expected, got one on {t.device}")
+
+
 def _a(t):
-    """Device address of a tensor (an integer: ctypes takes it as it is, a small call spends its time here)."""
-    if t is None:
-        return None
-    assert t.is_cuda, "device tensor expected"
-    return t.data_ptr()
+    """Address of a tensor (an integer: ctypes takes it as it is, a small call spends its time here)."""
+    return None if t is None else t.data_ptr()
 
 
 def _mat(t, dtype, rows, cols, what):
@@ -636,6 +641,7 @@ def _group_outputs(rows, cols, row8, row_descale, col8, col_descale):
 def fp8_quantize_block128(x, row8=None, row_descale=None, col8=None, col_descale=None, is_e5m2=False):
     """Codes of a bf16 matrix with one scale per 128 values of a row (row8, row_descale [rows, ceil(cols/128)]) and / or per
     128 values of a column (col8, col_descale [ceil(rows/128), cols]), from one read."""
+    _on(x, row8, row_descale, col8, col_descale)
     rows, cols = x.shape
     check(_L().cf_fp8_quantize_block128(_a(x), _mat(x, _bf16, rows, cols, "x"), rows, cols, is_e5m2,
                                         *_group_outputs(rows, cols, row8, row_descale, col8, col_descale), _s()))
@@ -643,6 +649,7 @@ def fp8_quantize_block128(x, row8=None, row_descale=None, col8=None, col_descale
 
 def swiglu_quantize_block128(gate, up, row8=None, row_descale=None, col8=None, col_descale=None):
     """fp8_quantize_block128 of silu(gate) * up (E4M3, no bf16 rounding in between); gate and up share a row pitch."""
+    _on(gate, up, row8, row_descale, col8, col_descale)
     rows, cols = gate.shape
     ld = _mat(gate, _bf16, rows, cols, "gate")
     if _mat(up, _bf16, rows, cols, "up") != ld:
@@ -653,6 +660,7 @@ def swiglu_quantize_block128(gate, up, row8=None, row_descale=None, col8=None, c
 
 def swiglu_backward_quantize_block128(gate, up, dh, row8=None, row_descale=None, col8=None, col_descale=None, is_e5m2=False):
     """Codes of the gradient of silu(gate) * up: [rows, 2 cols], d gate first, d up behind it; cols a multiple of 128."""
+    _on(gate, up, dh, row8, row_descale, col8, col_descale)
     rows, cols = gate.shape
     ld = _mat(gate, _bf16, rows, cols, "gate")
     if _mat(up, _bf16, rows, cols, "up") != ld:
@@ -664,6 +672,7 @@ def swiglu_backward_quantize_block128(gate, up, dh, row8=None, row_descale=None,
 def fp8_quantize_block128x128(w, w8, descale):
     """E4M3 codes of a weight [rows, cols], or of a stack [n, rows, cols], with one scale per 128x128 block
     (descale [..., ceil(rows/128), ceil(cols/128)])."""
+    _on(w, w8, descale)
     if w.dim() not in (2, 3) or w8.shape != w.shape or descale.dim() != w.dim():
         _refuse("weight, codes and descales: shapes differ")
     n = w.shape[0] if w.dim() == 3 else 1
@@ -684,6 +693,7 @@ def fp8_quantize_block128x128(w, w8, descale):
 def add_rmsnorm_quantize_block128(x, residual, scale, h, rms=None, normed=None, out8=None, descale=None, eps=1e-6):
     """h = bf16(x + residual), RMS norm of h with gain `scale`, codes and row-group descales of the normalised row (and / or
     its bf16 copy `normed`), in one pass. residual may be None (then h may be, too); h may be x or residual itself."""
+    _on(x, residual, scale, h, rms, normed, out8, descale)
     shape = rows, H = x.shape
     _dense(x, _bf16, shape, "x")
     _dense(residual, _bf16, shape, "residual")
@@ -706,6 +716,7 @@ def add_rmsnorm_backward_scratch_floats(rows, H):
 def add_rmsnorm_backward(dy, h, scale, rms, dh, dx, dscale=None, scratch=None, accumulate_dscale=False):
     """Gradient of the residual addition + RMS norm: dx (of x and of the residual alike) from dy and the gradient dh of the
     residual stream (or None); dscale float32 [H], stored or added to, or None. dx may be dy or dh itself."""
+    _on(dy, h, scale, rms, dh, dx, dscale, scratch)
     shape = rows, H = h.shape
     _dense(h, _bf16, shape, "h")
     _dense(dy, _bf16, shape, "dy")
@@ -730,6 +741,7 @@ def _output(out, M, N):
 def gemm_fp8_block128_nt(ctx, A8, a_descale, B8, b_descale, out, a_is_e5m2=False, accumulate=False):
     """out[M,N] (bf16 or float32) = A8[M,K] . B8[N,K]^T with a_descale [M, ceil(K/128)] and b_descale [ceil(N/128), ceil(K/128)]
     (128x128 blocks, weights) or [N, ceil(K/128)] (row groups; taken for blocks where the two shapes are the same, N = 1)."""
+    _on(A8, a_descale, B8, b_descale, out)
     (M, K), N = A8.shape, B8.shape[0]
     nb, kb = _blocks(N), _blocks(K)
     per = BLOCK if b_descale.shape[0] == nb else 1
@@ -742,6 +754,7 @@ def gemm_fp8_block128_nt(ctx, A8, a_descale, B8, b_descale, out, a_is_e5m2=False
 def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_descale, out, a_is_e5m2=False):
     """Rows [offsets[e], +counts[e]) of the compact A8 times expert e of the stacked B8 [E, N, K] (b_descale
     [E, ceil(N/128), ceil(K/128)]) into the same rows of the bf16 out; the other rows are left as they are."""
+    _on(counts, offsets, A8, a_descale, B8, b_descale, out)
     (T, K), (E, N, _) = A8.shape, B8.shape
     _dense(counts, _i32, (E,), "counts")
     _dense(offsets, _i32, (E,), "offsets")
@@ -761,6 +774,7 @@ def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_desc
 def gemm_fp8_block128_nn(ctx, A8, a_descale, B8_kn, b_descale, out, a_is_e5m2=False, accumulate=False):
     """Data gradient: out[M,N] = A8[M,K] . B8[K,N], the weight read from its forward cache ([out, in] = [K, N]) and block descales
     [ceil(K/128), ceil(N/128)] as they lie; A8 (the gradient) with row groups along K."""
+    _on(A8, a_descale, B8_kn, b_descale, out)
     (M, K), N = A8.shape, B8_kn.shape[1]
     ld_b, step = _scales(b_descale, _blocks(K), _blocks(N), "b_descale")
     if step != 1 and N > BLOCK:
@@ -773,6 +787,7 @@ def gemm_fp8_block128_nn(ctx, A8, a_descale, B8_kn, b_descale, out, a_is_e5m2=Fa
 def gemm_fp8_block128_dw(ctx, X8, x_descale, dY8, dy_descale, dW, x_is_e5m2=False, dy_is_e5m2=False, accumulate=False):
     """Weight gradient: dW[M,N] (float32 or bf16) = X8[T,M]^T . dY8[T,N] over T tokens, both with column groups of 128 tokens
     (descales [ceil(T/128), M] and [ceil(T/128), N])."""
+    _on(X8, x_descale, dY8, dy_descale, dW)
     (T, M), N = X8.shape, dY8.shape[1]
     kb = _blocks(T)
     check(_L().cf_gemm_fp8_block128_dw(ctx.handle, M, N, T, _a(X8), _mat(X8, _u8, T, M, "X8"), x_is_e5m2, _a(x_descale),

@@ -460,7 +460,9 @@ int cf_swiglu_quantize_e4m3_record(const void* d_gate, const void* d_up, int ld_
  * d[b * ld_block + c * ld_col]. NaN is ignored by the amax and coded as NaN; a group that holds an infinity gets descale +Inf
  * and contributes NaN. Any number of rows and columns and any pitch; 16-byte aligned inputs with pitches that are multiples
  * of 8 elements, and 8-byte aligned codes with pitches that are multiples of 8, take vector accesses. The GEMMs need
- * 16-byte aligned codes with pitches that are multiples of 16 (the columns behind a row's end are not read). */
+ * 16-byte aligned codes with pitches that are multiples of 16 (the columns behind a row's end are not read). The current
+ * device must be the one the memory (and the context) belongs to. Calls keep nothing from one to the next: any number of them
+ * may overlap on several streams and share a context. */
 
 /* bf16 [rows, cols] (pitch ld_x) -> codes with row groups and / or codes with column groups, from one read. A pair of
  * codes and descales is left out by passing NULL for both. */
@@ -511,7 +513,7 @@ int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_sca
 /* C[M,N] = sum over blocks b of 128 along K of da[m,b] * db[n,b] * sum_{k in b} A8[m,k] * B8[n,k]: block sums on the tensor
  * cores, scaled and added up in fp32, one rounding to the output type.
  * A8 [M, K] E4M3 or E5M2, row pitch lda; B8 [N, K] E4M3, row pitch ldb; both 16-byte aligned with pitches that are multiples
- * of 16 (CF_ERR_UNSUPPORTED otherwise), K any number. b_rows_per_scale: 128 (weights: db of row n at
+ * of 16 (CF_ERR_UNSUPPORTED otherwise), K any number (a sum over nothing is zero). b_rows_per_scale: 128 (weights: db of row n at
  * d[(n / 128) * ld_row + b * ld_block]) or 1 (row groups). C: bf16 or (out_fp32) float, pitch ldc, stored or (accumulate)
  * added to. No float atomics: results do not depend on timing. Few rows of A (and products with few tiles) take a form
  * that reads every weight once per 64 rows, with the contraction split over a cluster; the sums' order then differs. */
@@ -523,7 +525,8 @@ int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
  * the stacked weights [num_experts * N, K] (row pitch ldb), whose descales lie [ceil(N/128), ceil(K/128)] with row pitch
  * b_descale_ld_row and unit block stride, b_descale_stride apart per expert. All compact buffers have max_total_rows rows;
  * rows outside of them are never touched (a group is cut to them, one that starts outside is skipped), rows of no group are
- * left as they are. bf16 output, forward only. */
+ * left as they are; groups must not overlap. At most 65536 experts. bf16 output, forward only: the weight gradient of a ragged
+ * group would need its tokens padded to blocks of 128. */
 int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_rows, int N, int K, const int* d_counts,
                                     const int* d_offsets, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
                                     long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb,

@@ -74,18 +74,20 @@ def test_product_refusals(lib, err):
 
     def nt(ctx=ctx, M=300, N=256, K=256, A=P, lda=256, sa=P, B=P, ldb=256, sb=P, per=128, out=P, ldc=256, f32=0):
         return lib.cf_gemm_fp8_block128_nt(ctx, M, N, K, A, lda, 0, sa, 2, 1, B, ldb, sb, 2, 1, per, out, ldc, f32, 0, None)
-    for bad in (dict(ctx=None), dict(M=-1), dict(K=0), dict(A=None), dict(B=None), dict(sa=None), dict(sb=None), dict(out=None),
+    for bad in (dict(ctx=None), dict(M=-1), dict(K=-1), dict(A=None), dict(B=None), dict(sa=None), dict(sb=None), dict(out=None),
                 dict(lda=240), dict(ldb=240), dict(ldc=255), dict(per=64), dict(out=C.c_void_p(4098), f32=1), dict(sa=C.c_void_p(4097))):
         assert nt(**bad) == err.CF_ERR_INVALID_ARG, bad
     for bad in (dict(A=C.c_void_p(4104)), dict(B=C.c_void_p(4097)), dict(lda=264), dict(ldb=257)):
         assert nt(**bad) == err.CF_ERR_UNSUPPORTED, bad
+    assert nt(M=0x7fffffff) == err.CF_ERR_LIMIT
+    assert nt(K=0, A=None, B=None, sa=None, sb=None, ldc=255) == err.CF_ERR_INVALID_ARG
     g = lib.cf_gemm_fp8_block128_nt_grouped
 
     def grouped(E=2, T=300, counts=P, offsets=P, ldb=256, N=256):
         return g(ctx, E, T, N, 256, counts, offsets, P, 256, 0, P, 2, 1, P, ldb, P, 2, 4, P, N, None)
     for bad in (dict(E=0), dict(counts=None), dict(offsets=None), dict(ldb=255), dict(T=-1)):
         assert grouped(**bad) == err.CF_ERR_INVALID_ARG, bad
-    assert grouped(E=1 << 24, N=256) == err.CF_ERR_LIMIT
+    assert grouped(E=1 << 24, N=256) == err.CF_ERR_LIMIT and grouped(E=65537, N=16) == err.CF_ERR_LIMIT
     nn = lib.cf_gemm_fp8_block128_nn
     assert nn(ctx, 300, 256, 256, P, 256, 0, P, 2, 1, P, 255, P, 2, P, 256, 0, 0, None) == err.CF_ERR_INVALID_ARG
     assert nn(ctx, 300, 256, 256, P, 256, 0, P, 2, 1, P, 264, P, 2, P, 256, 0, 0, None) == err.CF_ERR_UNSUPPORTED
@@ -97,10 +99,11 @@ def test_product_refusals(lib, err):
 class _Dev:
     """Stands for a device tensor of a given shape: what the wrappers look at before they pass a pointer on."""
 
-    is_cuda = True
+    def __init__(self, t, device=0):
+        self.t, self.index = t, device
 
-    def __init__(self, t):
-        self.t = t
+    def get_device(self):
+        return self.index
 
     def __getattr__(self, name):
         return getattr(self.t, name)
@@ -119,6 +122,7 @@ def dev(*shape, dtype=torch.bfloat16, of=None):
 def test_wrappers_refuse_tensors_that_do_not_fit(monkeypatch):
     cfb = package()
     monkeypatch.setattr(cfb.ops, "_s", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     u8, f32 = torch.uint8, torch.float32
     ctx = type("Ctx", (), {"handle": P})()
 
@@ -161,3 +165,30 @@ def test_wrappers_refuse_tensors_that_do_not_fit(monkeypatch):
     refused(cfb.gemm_fp8_block128_nt_grouped, ctx, dev(2, dtype=torch.int64), c, A, da, E8, dev(2, 2, 2, dtype=f32), out)
     refused(cfb.gemm_fp8_block128_nt_grouped, ctx, c, c, A, da, dev(of=torch.empty((2, 300, 256), dtype=u8)[:, :256]), dev(2, 2, 2, dtype=f32), out)
     refused(cfb.gemm_fp8_block128_nt_grouped, ctx, c, c, A, da, E8, dev(2, 2, 2, dtype=f32), dev(300, 256, dtype=f32))
+
+
+def test_wrappers_refuse_tensors_of_another_device(monkeypatch):
+    """The call goes to the current device's stream: a tensor on the CPU or on another GPU is refused, by every operator."""
+    cfb = package()
+    monkeypatch.setattr(cfb.ops, "_s", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    ctx = type("Ctx", (), {"handle": P})()
+    u8, f32 = torch.uint8, torch.float32
+    x, g, c8, d, out = dev(256, 256), dev(256), dev(256, 256, dtype=u8), dev(2, 2, dtype=f32), dev(256, 256)
+    rd, cd, v, i = dev(256, 2, dtype=f32), dev(2, 256, dtype=f32), dev(256, dtype=f32), dev(1, dtype=torch.int32)
+    W, e8, ed = dev(2, 256, 256), dev(1, 256, 256, dtype=u8), dev(1, 2, 2, dtype=f32)
+    rd2, c82 = dev(256, 4, dtype=f32), dev(256, 512, dtype=u8)
+    scratch = dev(1 << 20, dtype=f32)
+    calls = ((cfb.fp8_quantize_block128, (x, c8, rd, c8, cd)), (cfb.swiglu_quantize_block128, (x, x, c8, rd, c8, cd)),
+             (cfb.swiglu_backward_quantize_block128, (x, x, x, c82, rd2)), (cfb.fp8_quantize_block128x128, (x, c8, d)),
+             (cfb.add_rmsnorm_quantize_block128, (x, x, g, x, v, x, c8, rd)), (cfb.add_rmsnorm_backward, (x, x, g, v, x, x, v, scratch)),
+             (cfb.gemm_fp8_block128_nt, (ctx, c8, rd, c8, d, out)), (cfb.gemm_fp8_block128_nt_grouped, (ctx, i, i, c8, rd, e8, ed, out)),
+             (cfb.gemm_fp8_block128_nn, (ctx, c8, rd, c8, d, out)), (cfb.gemm_fp8_block128_dw, (ctx, c8, cd, c8, cd, out)))
+    for fn, args in calls:
+        for k, a in enumerate(args):
+            if isinstance(a, _Dev):
+                for other in (-1, 1):
+                    moved = args[:k] + (_Dev(a.t, other),) + args[k + 1:]
+                    with pytest.raises(cfb.CanopyError) as e:
+                        fn(*moved)
+                    assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG and "device" in str(e.value), (fn.__name__, k)

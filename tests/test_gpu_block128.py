@@ -510,6 +510,89 @@ def test_empty_sizes_do_nothing(cfb, ctx):
     assert dg.eq(1).all()
 
 
+def test_empty_contraction_is_zero(cfb, ctx):
+    for dtype in (torch.bfloat16, torch.float32):
+        out, raw = pitched(5, 100, dtype, 3)
+        out.fill_(2.0)
+        kept = raw.clone()
+        A, da, B, db = (torch.empty(s, dtype=t, device="cuda") for s, t in (((5, 0), torch.uint8), ((5, 0), torch.float32), ((100, 0), torch.uint8), ((1, 0), torch.float32)))
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out, accumulate=True)
+        assert torch.equal(raw, kept)
+        cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+        assert out.eq(0).all()
+        out.fill_(2.0)
+        X, dx, Y, dy = (torch.empty(s, dtype=t, device="cuda") for s, t in (((0, 5), torch.uint8), ((0, 5), torch.float32), ((0, 100), torch.uint8), ((0, 100), torch.float32)))
+        cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, out)
+        assert out.eq(0).all()
+        out.fill_(2.0)
+        assert torch.equal(raw, kept)                    # nothing beside the matrix was written
+
+
+@pytest.mark.parametrize("pad,offset", [(1, 0), (8, 8), (3, 5)])
+def test_swiglu_pitches_and_alignments(cfb, pad, offset):
+    rows, cols = 141, 256
+    (gate, _), (up, _), (dh, _) = (pitched(rows, cols, torch.bfloat16, pad, offset) for _ in range(3))
+    for i, t in enumerate((gate, up, dh)):
+        t.copy_(normal((rows, cols), 140 + i))
+    even = [t.contiguous() for t in (gate, up, dh)]
+
+    def run(g, u, d, view):
+        q, qc = view(cols), view(cols)
+        rd, cd = torch.empty((rows, 2), device="cuda"), torch.empty((2, cols), device="cuda")
+        cfb.swiglu_quantize_block128(g, u, q, rd, qc, cd)
+        b, bc = view(2 * cols), view(2 * cols)
+        bd, bcd = torch.empty((rows, 4), device="cuda"), torch.empty((2, 2 * cols), device="cuda")
+        cfb.swiglu_backward_quantize_block128(g, u, d, b, bd, bc, bcd)
+        alone, ad = view(2 * cols), torch.empty((rows, 4), device="cuda")
+        cfb.swiglu_backward_quantize_block128(g, u, d, alone, ad)
+        calone, cad = view(2 * cols), torch.empty((2, 2 * cols), device="cuda")
+        cfb.swiglu_backward_quantize_block128(g, u, d, col8=calone, col_descale=cad)
+        assert torch.equal(alone, b) and torch.equal(ad, bd) and torch.equal(calone, bc) and torch.equal(cad, bcd)
+        return q, rd, qc, cd, b, bd, bc, bcd
+
+    odd = run(gate, up, dh, lambda c: pitched(rows, c, torch.uint8, pad, offset)[0])
+    plain = run(*even, lambda c: torch.empty((rows, c), dtype=torch.uint8, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(odd, plain))
+
+
+def test_offsets_beyond_32_bits(cfb, ctx):
+    """Rows whose elements lie more than 2^32 apart from the first one: quantisers, both forms of the product, all outputs."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    rows, cols, far = 4, 256, 1_600_000_000              # 3 * far elements > 2^32
+    big = torch.empty(rows * far, dtype=torch.uint8, device="cuda")
+    q = big.view(rows, far)[:, :cols]
+    x = normal((rows, cols), 150)
+    rd, cd = torch.empty((rows, 2), device="cuda"), torch.empty((1, cols), device="cuda")
+    cfb.fp8_quantize_block128(x, q, rd)
+    want, _ = plain_codes(x, 1, False)
+    assert torch.equal(q, want)
+    B, db = coded(384, cols, 151, G, G)
+    out = torch.empty((rows, 384), device="cuda")
+    cfb.gemm_fp8_block128_nt(ctx, q, rd, B, db, out)     # narrow form, A far apart
+    check_product(out, value64(q, rd, False, 1, G), value64(B, db, False, G, G).t(), cols)
+    cfb.fp8_quantize_block128(x, col8=q, col_descale=cd)
+    want, _ = plain_codes(x, 0, False)
+    assert torch.equal(q, want)
+    del big, q
+    M, N, far = 300, 384, 16_000_000                     # 299 * far elements > 2^32
+    big = torch.empty(M * far, dtype=torch.bfloat16, device="cuda")
+    out = big.view(M, far)[:, :N]
+    A, da = coded(M, cols, 152, 1, G)
+    for n in (M, 40):                                    # wide and narrow form, output rows far apart
+        cfb.gemm_fp8_block128_nt(ctx, A[:n], da[:n], B, db, out[:n] if n == M else out[M - n:])
+        check_product(out[:n] if n == M else out[M - n:], value64(A[:n], da[:n], False, 1, G), value64(B, db, False, G, G).t(), cols)
+    xin = out[:, :cols]
+    xin.copy_(normal((M, cols), 153))
+    q = torch.empty((M, cols), dtype=torch.uint8, device="cuda")
+    rd = torch.empty((M, 2), device="cuda")
+    cfb.fp8_quantize_block128(xin, q, rd)                # input rows far apart
+    want, d = plain_codes(xin, 1, False)
+    assert torch.equal(q, want) and torch.equal(rd, d)
+    ctx.poll_status()
+
+
 # ---------------------------------------------------------------- run together
 def rel(a, b):
     a, b = a.detach().double(), b.detach().double()
