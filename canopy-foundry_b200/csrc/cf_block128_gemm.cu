@@ -42,8 +42,8 @@ constexpr int SB = 128;                 // elements of K that share a scale == B
 constexpr int NUM_THREADS = 384;        // warpgroup 0: producer, two MMA issuers, scales; warpgroups 1 and 2: promotion + epilogue
 constexpr int EPI_WARPS = 8;
 // Registers: the launch gives every thread kLaunchRegs; warpgroup 0 hands most of its share to the two others, which hold 128
-// accumulators a thread. 56 x 128 + 224 x 256 = 168 x 384: the shares add up to what the launch has (the host checks that).
-constexpr int kLaunchRegs = 168, kLeanRegs = 56, kWideRegs = 224;
+// accumulators a thread. 40 x 128 + 232 x 256 = 168 x 384: the shares add up to what the launch has (the host checks that).
+constexpr int kLaunchRegs = 168, kLeanRegs = 40, kWideRegs = 232;
 static_assert(kLeanRegs * 128 + kWideRegs * 256 <= kLaunchRegs * NUM_THREADS, "register shares");
 constexpr int TMEM_COLS = 512;          // two 128x256 fp32 block sums per CTA
 constexpr int C_STAGING = EPI_WARPS * C_BOX_BYTES;
@@ -142,6 +142,20 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// One lane of the (converged) warp. Inside such a branch the compiler keeps descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// Ties a read's registers to this place: the read has been waited for, and what follows uses them from here on only.
+__device__ __forceinline__ void pin(uint32_t (&v)[32]) {
+    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
 // ---- tiles ----------------------------------------------------------------------------------------------------------
 struct Tile {
     int row0;        // first row of A / C
@@ -320,9 +334,12 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     } else if (warp == 1 || warp == 3) {
         // ------------------------------------------------------------ MMA issuers (leader CTA only)
         // Warp 1 issues the even blocks, warp 3 the odd ones, each into its own TMEM buffer: the two sequences do not depend on
-        // each other, and while one thread waits for barriers and commits, the other one's MMAs keep the tensor cores fed.
-        // One issuer for both left them idle for half of the time (1030 clocks a block where its MMAs take 500).
-        if (lane == 0 && leader) {
+        // each other, and while one warp waits for barriers and commits, the other one's MMAs keep the tensor cores fed. One
+        // issuer for both left them idle for half of the time (1030 clocks a block where its MMAs take 500). The warps stay
+        // converged and one elected lane issues: descriptors then live in uniform registers, and a block's four MMAs and the
+        // commit take 160 clocks to issue instead of 520 from a lane of its own.
+        if (leader) {
+            const bool elected = elect_one();
             const int mine = warp >> 1;                      // 0: even, 1: odd
             const int blocks = unit < total_tiles ? ((total_tiles - unit - 1) / n_units + 1) * k_iters : 0;
             const uint32_t idesc = make_idesc(p.a_e5m2, p.b_e5m2, TM, BN, p.a_mn, p.b_mn);
@@ -330,27 +347,32 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // further in an MN-major one
             const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
             const uint32_t tmem_d = tmem_base + mine * BN, tempty = tempty_bar + 8 * mine;
+            const uint64_t desc_a0 = make_smem_desc(smem_a), desc_b0 = make_smem_desc(smem_b);
             int s = mine;
             uint32_t phase = 0, t_phase = 1;
             bool ok = true;
             for (int it = mine; it < blocks; it += 2) {
                 if (!mbar_wait(tempty, t_phase, s_abort) || !mbar_wait(full_bar + 8 * s, phase, s_abort)) { ok = false; break; }
                 tcgen05_fence_after();
-                const uint64_t adesc = make_smem_desc(smem_a + s * A_STAGE);
-                const uint64_t bdesc = make_smem_desc(smem_b + s * B_STAGE);
+                const uint64_t adesc = desc_a0 + static_cast<uint32_t>(s * (A_STAGE >> 4));
+                const uint64_t bdesc = desc_b0 + static_cast<uint32_t>(s * (B_STAGE >> 4));
+                if (elected) {
 #pragma unroll
-                for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                    if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
-                    else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                        else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                    }
+                    // the stage may be filled again, and the block's sums may be read (in both CTAs of a pair)
+                    if (PAIR) tcgen05_commit_pair(done_bar + 8 * s); else tcgen05_commit(done_bar + 8 * s);
                 }
-                // the stage may be filled again, and the block's sums may be read (in both CTAs of a pair)
-                if (PAIR) tcgen05_commit_pair(done_bar + 8 * s); else tcgen05_commit(done_bar + 8 * s);
+                __syncwarp();
                 t_phase ^= 1u;
                 s += 2;
                 if (s >= STAGES) { s -= STAGES; phase ^= 1u; }
             }
-            if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x600 | 1); }
-            if (*s_abort || !ok) {
+            if (!ok && elected && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x600 | 1); }
+            __syncwarp();
+            if ((*s_abort || !ok) && elected) {
                 if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar + 8 * mine) : "memory");
                 else tcgen05_commit(drain_bar + 8 * mine);
                 mbar_wait(drain_bar + 8 * mine, 0, s_abort + 1, DRAIN_NS);
@@ -449,6 +471,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             tmem_ld32(tcol + (it & 1) * BN, v[0]);
                         }
                     }
+                    pin(v[c & 1]);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         uint64_t x0 = pack_f2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1]));
