@@ -1,11 +1,14 @@
 // Residual addition + RMS norm with block-scaled FP8 output, and the gradient of the pair.
 //
 //   forward   h = bf16(x + residual);  rms = sqrt(mean(h^2) + eps);  y = (h / rms) * scale
-//             per 128 values of y: a = max(max|y|, 1e-12), descale = a / 448, code = e4m3(y * (448 / a))
+//             per 128 values of y: a = max(max|y|, 1e-12), descale = a / 448, code = e4m3(y * 448 / a)
 //   backward  u = dy * scale;  dx = (u - h * sum(u h) / (H rms^2)) / rms + dh;  dscale = sum over rows of dy * h / rms
 //
 // h is rounded to bf16 before the norm reads it: it is the residual stream the next layers and the backward pass see. y is
-// NOT rounded to bf16 on its way to the codes (one rounding, descales from fp32); the optional bf16 copy of y is.
+// NOT rounded to bf16 on its way to the codes (one rounding, descales from fp32); the optional bf16 copy of y is. The codes do
+// not depend on rms: with t = h * scale (exact in fp32, 16 bits) and m = max|t| over the group, y * 448 / a = t * 448 / m. The
+// quotient is taken correctly rounded, exact where it is representable: it lands exactly between two codes about once in a
+// thousand values, and a rounded factor would send such a value to either side.
 // Sums, rms and descales are fp32.
 //
 // Both are streams: forward 2+2 B in, 2+1 B out per element (7), backward 2+2+2 in, 2 out (8). A row lives in the registers
@@ -129,21 +132,26 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
         const float rms = sqrtf(__fdiv_rn(total, static_cast<float>(p.H)) + p.eps);
         if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
         const float inv = __fdiv_rn(1.0f, rms);
-        float amax[NV];                                 // of the group of 128 that this half-warp holds in vector i
-        float y[NV][8];
+        float amax[NV];                                 // of t over the group of 128 that this half-warp holds in vector i
+        float t[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int vi = threadIdx.x + blockDim.x * i;
             float g[8];
-            unpack8(v[i], y[i]);
+            unpack8(v[i], t[i]);
             unpack8(vi < nv ? load8<VEC>(p.gain + vi * 8, p.H - vi * 8) : make_uint4(0u, 0u, 0u, 0u), g);
             amax[i] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                y[i][e] = y[i][e] * inv * g[e];
-                amax[i] = fmaxf(amax[i], fabsf(y[i][e]));
+                t[i][e] *= g[e];
+                amax[i] = fmaxf(amax[i], fabsf(t[i][e]));
             }
-            if (p.normed && vi < nv) store8<VEC>(p.normed + base + vi * 8, pack8(y[i]), p.H - vi * 8);
+            if (p.normed && vi < nv) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = t[i][e] * inv;
+                store8<VEC>(p.normed + base + vi * 8, pack8(y), p.H - vi * 8);
+            }
         }
         if (p.out8) {                                   // kernel-uniform
 #pragma unroll
@@ -157,17 +165,24 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
 #pragma unroll
             for (int i = 1; i < NV; ++i)
                 if (cg == i) mine = amax[i];
-            mine = fmaxf(mine, 1e-12f);
-            const float scale = __fdiv_rn(448.0f, mine);
+            mine = fmaxf(mine, 1e-12f * rms);           // the floor of max|y|
+            // 448 / m in two parts, 8 significant bits and the rest: t * hi is exact, fma(t, lo, t * hi) the rounded quotient
+            const float quot = __fdiv_rn(448.0f, mine);
+            const float s_hi = __uint_as_float(__float_as_uint(quot) & 0xffff0000u);
+            const float rest = fmaf(fmaf(-quot, mine, 448.0f), quot * (1.0f / 448.0f), quot - s_hi);
+            const float s_lo = isfinite(rest) ? rest : 0.0f;        // a group with an infinity: the quotient is 0
             const int my_group = (threadIdx.x + blockDim.x * cg) / 16;
-            if (cg < NV && my_group * 16 < nv) p.descale[row * p.d_row + my_group * p.d_blk] = __fdiv_rn(mine, 448.0f);
+            if (cg < NV && my_group * 16 < nv) p.descale[row * p.d_row + my_group * p.d_blk] = __fdiv_rn(mine * inv, 448.0f);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int vi = threadIdx.x + blockDim.x * i;
-                const float s = __shfl_sync(0xffffffffu, scale, (lane & 16) | i);
+                const float hi = __shfl_sync(0xffffffffu, s_hi, (lane & 16) | i), lo = __shfl_sync(0xffffffffu, s_lo, (lane & 16) | i);
                 if (vi < nv) {
-                    const uint32_t q0 = cvt_fp8x4<false>(y[i][0] * s, y[i][1] * s, y[i][2] * s, y[i][3] * s);
-                    const uint32_t q1 = cvt_fp8x4<false>(y[i][4] * s, y[i][5] * s, y[i][6] * s, y[i][7] * s);
+                    float q[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[e] = fmaf(t[i][e], lo, t[i][e] * hi);
+                    const uint32_t q0 = cvt_fp8x4<false>(q[0], q[1], q[2], q[3]);
+                    const uint32_t q1 = cvt_fp8x4<false>(q[4], q[5], q[6], q[7]);
                     uint8_t* o = p.out8 + row * p.ld_out8 + vi * 8;
                     if (VEC && p.vec8) {
                         *reinterpret_cast<uint2*>(o) = make_uint2(q0, q1);

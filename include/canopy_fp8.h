@@ -452,7 +452,8 @@ int cf_swiglu_quantize_e4m3_record(const void* d_gate, const void* d_up, int ld_
 /* ------------------------------------------------------------------ block-scaled FP8 (one scale per 128 values)
  *
  * No counterpart in the reference, which scales per tensor; the formulas generalise kernels/fp8.cu:34-49 to groups of 128:
- *   a = max(max|v| over the group, 1e-12), descale = a / FMAX, code = fp8(v * (FMAX / a)),  FMAX = 448 (E4M3) or 57344 (E5M2)
+ *   a = max(max|v| over the group, 1e-12), descale = a / FMAX, code = fp8(v * FMAX / a),  FMAX = 448 (E4M3) or 57344 (E5M2)
+ * (for bf16 values v * FMAX / a is rounded once before it is rounded to the code, ties between two codes included)
  * Groups: 1x128 along a row (operands contracted along the row), 128x1 down a column (operands of the weight gradient,
  * contracted over tokens), 128x128 blocks (weights). The last group of a row or column may be shorter. Descales are fp32 and
  * addressed by strides in elements, so they may lie [rows, groups], [groups, rows] (what coalesces best in the GEMM) or

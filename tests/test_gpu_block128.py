@@ -73,13 +73,21 @@ def check_groups(codes, descale, v, dim, e5m2, slack):
     assert err.le(bound).all(), float((err - bound).max())
 
 
+def nearest64(v, e5m2):
+    """Codes of the 64-bit values: round to nearest, ties to even, from the format's definition."""
+    mant, low = (2, -14) if e5m2 else (3, -6)
+    _, e = torch.frexp(v)
+    step = torch.ldexp(torch.ones_like(v), torch.clamp(e - 1, min=low) - mant)
+    return torch.clamp(torch.round(v / step) * step, -FMAX[e5m2], FMAX[e5m2]).to(TYPE[e5m2]).view(torch.uint8)
+
+
 def plain_codes(x, dim, e5m2):
-    """The same fp32 operations in torch: bit-exact codes and descales of a bf16 matrix. (Quotients are taken in 64 bits and
-    rounded, which is the IEEE fp32 quotient; torch's own division by or of a scalar goes through a rounded reciprocal.)"""
-    a, per = groups64(x.double(), dim)
+    """Codes and descales of a bf16 matrix from the 64-bit quotients. (v * FMAX is exact in 64 bits and the quotient of an 11-bit
+    and an 8-bit number is either representable or further than 2^-20 from every code's border: no double rounding.)"""
+    v = x.double()
+    a, per = groups64(v, dim)
     a, per = a.float().double(), per.float().double()
-    q = (x.float() * (FMAX[e5m2] / a).float()).clamp(-FMAX[e5m2], FMAX[e5m2]).to(TYPE[e5m2])
-    return q.view(torch.uint8), (per / FMAX[e5m2]).float()
+    return nearest64(v * FMAX[e5m2] / a, e5m2), (per / FMAX[e5m2]).float()
 
 
 # ---------------------------------------------------------------- quantiser
@@ -154,9 +162,9 @@ def test_quantise_weight_blocks_bit_exact(cfb, shape):
     cfb.fp8_quantize_block128x128(w, w8, d)
     for i in range(cdiv(shape[-2], G)):
         for j in range(cdiv(shape[-1], G)):
-            part = w[..., i * G:(i + 1) * G, j * G:(j + 1) * G].float()
+            part = w[..., i * G:(i + 1) * G, j * G:(j + 1) * G].double()
             a = part.abs().amax((-2, -1), keepdim=True).clamp(min=1e-12)
-            q = (part * (448.0 / a.double()).float()).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+            q = nearest64(part * 448.0 / a, False)
             assert torch.equal(w8[..., i * G:(i + 1) * G, j * G:(j + 1) * G], q)
             assert torch.equal(d[..., i, j], (a.double() / 448.0).float()[..., 0, 0])
 
@@ -237,6 +245,15 @@ def test_add_rmsnorm_quantise(cfb, rows, H, residual):
     assert (rms.double() - rms64).abs().le(slack * rms64).all()
     assert (normed.double() - y).abs().le((2.0 ** -8 + slack) * y.abs() + 1e-38).all()
     check_groups(out8, d, y, 1, False, slack)
+    # the codes are the correctly rounded t * 448 / max|t| with t = h * gain, exact ties included (a 19-bit over a 16-bit number:
+    # representable or 2^-38 from a border at least, and 64 bits tell those apart)
+    t = want_h.double() * gain.double()
+    a, _ = groups64(t, 1)
+    same = out8 == nearest64(t * 448.0 / a, False)
+    # the kernel's quotient carries an error of half a unit of fp32: a border closer than 2^-23 may be on the other side
+    off = (t * 448.0 / a)[~same]
+    near = torch.minimum((nearest64(off * (1 + 2.0 ** -22), False) != nearest64(off * (1 - 2.0 ** -22), False)).double(), torch.ones_like(off))
+    assert near.bool().all(), int((~same).sum())
     # in place: h may be the residual, or x; the codes alone and the bf16 row alone are the same
     for into in ("r", "x"):
         xx, rr = x.clone(), r.clone()
