@@ -352,18 +352,20 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             uint32_t phase = 0, t_phase = 1;
             bool ok = true;
             for (int it = mine; it < blocks; it += 2) {
-                if (!mbar_wait(tempty, t_phase, s_abort) || !mbar_wait(full_bar + 8 * s, phase, s_abort)) { ok = false; break; }
-                tcgen05_fence_after();
                 const uint64_t adesc = desc_a0 + static_cast<uint32_t>(s * (A_STAGE >> 4));
                 const uint64_t bdesc = desc_b0 + static_cast<uint32_t>(s * (B_STAGE >> 4));
-                if (elected) {
+                if (elected && ok) {                         // a wait that gave up: the loop runs out without doing anything
+                    ok = mbar_wait(tempty, t_phase, s_abort) && mbar_wait(full_bar + 8 * s, phase, s_abort);
+                    if (ok) {
+                        tcgen05_fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-                        if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
-                        else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                            if (PAIR) umma_f8_pair(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                            else umma_f8(tmem_d, adesc + a_step * kk, bdesc + b_step * kk, idesc, kk != 0 ? 1u : 0u);
+                        }
+                        // the stage may be filled again, and the block's sums may be read (in both CTAs of a pair)
+                        if (PAIR) tcgen05_commit_pair(done_bar + 8 * s); else tcgen05_commit(done_bar + 8 * s);
                     }
-                    // the stage may be filled again, and the block's sums may be read (in both CTAs of a pair)
-                    if (PAIR) tcgen05_commit_pair(done_bar + 8 * s); else tcgen05_commit(done_bar + 8 * s);
                 }
                 __syncwarp();
                 t_phase ^= 1u;
@@ -427,8 +429,9 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const uint64_t store_policy = l2_policy_evict_first();
         int it = 0, st = 0;                                // block, its stage
         uint32_t d_phase = 0;
-        bool ok = true;
-        for (int tile = unit; ok && tile < total_tiles; tile += n_units) {
+        bool ok = true;                                    // per lane: one whose wait gave up goes on without waiting, so that the
+                                                           // warp stays together (the results are reported as invalid)
+        for (int tile = unit; tile < total_tiles; tile += n_units) {
             const Tile tc_ = tile_at(p, counts, offsets, tile, m_blocks, TM);
             const int warp_row = tc_.row0 + static_cast<int>(cta_rank) * BM + quarter * 32;
             const int wcol = tc_.n0 + half * 128;          // first column of this warp
@@ -439,8 +442,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // is folded in, the next one is on its way. A buffer goes back as soon as its last chunk is in registers.
             const uint32_t tcol = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
             uint32_t v[2][32];
-            ok = mbar_wait(done_bar + 8 * st, d_phase, s_abort);
-            if (!ok) break;
+            ok = ok && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
             tcgen05_fence_after();
             tmem_ld32(tcol + (it & 1) * BN, v[0]);
             for (int kb = 0; kb < k_iters; ++kb) {
@@ -465,8 +467,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         ++it;
                         if (++st == STAGES) { st = 0; d_phase ^= 1u; }
                         if (kb + 1 < k_iters) {
-                            ok = mbar_wait(done_bar + 8 * st, d_phase, s_abort);
-                            if (!ok) break;
+                            ok = ok && mbar_wait(done_bar + 8 * st, d_phase, s_abort);
                             tcgen05_fence_after();
                             tmem_ld32(tcol + (it & 1) * BN, v[0]);
                         }
@@ -485,13 +486,11 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         acc[c * 16 + j + 1] = fma_f2(x1, s2, acc[c * 16 + j + 1]);
                     }
                 }
-                if (!ok) break;
                 if (BVEC) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(done);
                 }
             }
-            if (!ok) break;
             // ---- the tile's 32 rows x 128 columns of this warp leave
             const bool f32 = p.out_kind == OUT_F32 || p.out_kind == OUT_F32_ADD;
             // a box may only leave whole: in the ragged form its rows must all belong to the group
@@ -564,7 +563,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
         }
         if (lane == 0) bulk_wait_all();
-        if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x700 | 1); }
+        if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0x700 | 1); }
     }
 
     tcgen05_fence_before();
@@ -773,7 +772,7 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
             __syncwarp();
             if (++slot == C::AHEAD) slot = 0;
             fetch();
-            if (!mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort)) { ok = false; break; }
+            ok = ok && mbar_wait(tfull_bar + 8 * buf, (it >> 1) & 1, s_abort);     // see the wide form
             tcgen05_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
             const uint64_t w2 = pack_f2(w, w);
@@ -802,7 +801,7 @@ k_gemm_b128_narrow(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         }
         cp_async_wait_all();
-        if (!ok && lane == 0 && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xa00 | 1); }
+        if (!ok && !*s_abort) { *s_abort = 1; atomicExch(p.d_status, 0xa00 | 1); }
     }
 
     tcgen05_fence_before();
