@@ -16,6 +16,8 @@
 // barrier per row joins the row sum (two copies of the partial sums alternate, so the next row needs no second barrier).
 // The gain's gradient is summed per block over the block's rows in registers, written as one partial row per block and
 // added up in block order by a second launch: no atomics, so the result does not depend on timing.
+#include <type_traits>
+
 #include "cf_common.cuh"
 #include "cf_internal.cuh"
 
@@ -89,7 +91,9 @@ struct NormParams {
     int vec8;
 };
 
-// x, res and h may be the same memory (every thread reads its own elements before it writes them): no __restrict__.
+// x, res and h may be the same memory (every thread reads its own elements before it writes them, and a row belongs to one
+// block): no __restrict__. A row's loads of x and of the residual are all issued before either is used: 16384 x 4096 takes
+// 78 us (0.92 of the measured copy rate), 89 with the residual's loads behind the use of x's.
 template <int NV, bool VEC>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
     __shared__ float s_sum[2][32];
@@ -97,26 +101,26 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
     int par = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
         const long long base = row * p.H;
-        uint4 v[NV];
+        uint4 v[NV], res[NV];
         float acc = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int vi = threadIdx.x + blockDim.x * i;
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (vi < nv) v[i] = load8<VEC>(p.x + base + vi * 8, p.H - vi * 8);
+            v[i] = res[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (vi < nv) {
+                v[i] = load8<VEC>(p.x + base + vi * 8, p.H - vi * 8);
+                if (p.res) res[i] = load8<VEC>(p.res + base + vi * 8, p.H - vi * 8);
+            }
         }
         if (p.res) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int vi = threadIdx.x + blockDim.x * i;
-                if (vi < nv) {
-                    float a[8], b[8];
-                    unpack8(v[i], a);
-                    unpack8(load8<VEC>(p.res + base + vi * 8, p.H - vi * 8), b);
+                float a[8], b[8];
+                unpack8(v[i], a);
+                unpack8(res[i], b);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) a[e] += b[e];
-                    v[i] = pack8(a);
-                }
+                for (int e = 0; e < 8; ++e) a[e] += b[e];
+                v[i] = pack8(a);
             }
         }
 #pragma unroll
@@ -208,9 +212,11 @@ struct NormGradParams {
     int rows, H;
 };
 
-// dx may be the same memory as dy or dh. PREFETCH: the next row's loads are issued before this row's barrier.
-template <int NV, bool VEC, int MAXT, bool PREFETCH>
-__global__ void __launch_bounds__(MAXT, MAXT <= 512 && PREFETCH ? 2 : 1) k_add_rmsnorm_grad(const NormGradParams p) {
+// dx may be the same memory as dy or dh. The next row's loads are issued before this row's barrier, except with four vectors a
+// thread, which leave no registers for it. Two resident blocks with one vector, one block (128 registers a thread) otherwise.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) k_add_rmsnorm_grad(const NormGradParams p) {
+    constexpr bool PREFETCH = NV <= 2;
     __shared__ float s_sum[2][32];
     const int nv = (p.H + 7) / 8;
     float dg[NV][8];
@@ -291,6 +297,7 @@ __global__ void __launch_bounds__(1024) k_sum_partials(const float* __restrict__
     const int c = blockIdx.x * 32 + lane;
     float t = 0.0f;
     if (c < H)
+#pragma unroll 8
         for (int r = warp; r < n; r += 32) t += partial[static_cast<long long>(r) * H + c];
     s[warp][lane] = t;
     __syncthreads();
@@ -310,17 +317,24 @@ int threads_for(int nv, int per_thread) {
     return (t + 31) / 32 * 32;
 }
 
-// Vectors of 8 a thread holds. Forward: four; with few rows as few as possible, so that a row is spread over more threads (one
-// row of 4096: 512 threads). Gradient: one, which leaves registers for the next row's loads; four for rows beyond 8192 elements
-// (a block has 1024 threads at most).
-constexpr int kFwdVec = 4;
-constexpr int grad_vec(int H) { return H <= 8192 ? 1 : 4; }
+// Vectors of 8 a thread holds. Forward: four, which keeps the most loads in flight; fewer where a row has too few threads then.
+// Rows of 2048 and shorter: two / four 80.5 / 85.5 us (32768 x 2048); up to four short rows an SM: 4.0 / 4.5 us (512 x 4096;
+// 1024 x 4096: 6.9 / 5.8); a row an SM: as few as possible (one row of 4096: 512 threads). Gradient: blocks of
+// 512 threads at most, which leave registers for the next row's loads: one up to 4096 elements, two up to 8192 (4096 x 8192:
+// 52 us; one in blocks of 1024 threads 55), four beyond. Up to 4096 two or three smaller blocks of two vectors, with or without
+// loads ahead, take the same time or longer (8192 x 4096: 49 to 71 us; as it is 49).
+int fwd_vec(int rows, int H) {
+    if (rows <= sm_count()) return H <= 8192 ? 1 : 2;
+    return H <= 2048 || (H <= 4096 && rows <= 4 * sm_count()) ? 2 : 4;
+}
+constexpr int grad_vec(int H) { return H <= 4096 ? 1 : H <= 8192 ? 2 : 4; }
 
 template <int NV, bool VEC>
 int launch_forward(const NormParams& p, cudaStream_t st) {
     const int t = threads_for((p.H + 7) / 8, NV);
-    // resident blocks, two rounds of them at most: the rest of the rows is walked by the blocks
-    const long long most = static_cast<long long>(sm_count()) * (2048 / t < 16 ? 2048 / t : 16);
+    // three full rounds of the resident blocks (64 registers a thread) at most: the rest of the rows is walked by the blocks.
+    // Rounds of 2048 threads, 2.25 of them for 7168 elements: 81 us instead of 75 (9000 rows)
+    const long long most = static_cast<long long>(sm_count()) * 3 * (1024 / t);
     const long long grid = p.rows < most ? p.rows : most;
     k_add_rmsnorm<NV, VEC><<<static_cast<unsigned>(grid), t, 0, st>>>(p);
     CF_LAUNCH_CHECK("add_rmsnorm");
@@ -329,7 +343,7 @@ int launch_forward(const NormParams& p, cudaStream_t st) {
 
 int grad_blocks(int rows, int H) {
     const int t = threads_for((H + 7) / 8, grad_vec(H));
-    const int b = kBwdBlocks * (grad_vec(H) > 1 ? 1 : t <= 128 ? 8 : t <= 256 ? 4 : t <= 512 ? 2 : 1);
+    const int b = kBwdBlocks * (grad_vec(H) > 1 ? 1 : t <= 128 ? 8 : t <= 256 ? 4 : 2);
     return b < rows ? b : rows;
 }
 
@@ -368,9 +382,9 @@ int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_
     const bool vec = H % 8 == 0 && aligned(d_x, 16) && aligned(d_residual_or_null, 16) && aligned(d_scale, 16) &&
                      aligned(d_h_or_null, 16) && aligned(d_normed_or_null, 16);
     cudaStream_t st = as_stream(stream);
-    if (!vec) return launch_forward<kFwdVec, false>(p, st);
-    if (rows <= sm_count()) return H <= 8192 ? launch_forward<1, true>(p, st) : launch_forward<2, true>(p, st);
-    return launch_forward<kFwdVec, true>(p, st);
+    if (!vec) return launch_forward<4, false>(p, st);
+    const int nv = fwd_vec(rows, H);
+    return nv == 1 ? launch_forward<1, true>(p, st) : nv == 2 ? launch_forward<2, true>(p, st) : launch_forward<4, true>(p, st);
 }
 
 size_t cf_add_rmsnorm_backward_scratch_floats(int rows, int H) {
@@ -406,16 +420,14 @@ int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_sca
     p.rows = rows; p.H = H;
     const bool vec = H % 8 == 0 && aligned(d_dy, 16) && aligned(d_h, 16) && aligned(d_scale, 16) && aligned(d_dh_or_null, 16) && aligned(d_dx, 16);
     const int nv = grad_vec(H), t = threads_for((H + 7) / 8, nv), blocks = grad_blocks(rows, H);
-    if (nv == 1 && t <= 512) {
-        if (vec) k_add_rmsnorm_grad<1, true, 512, true><<<blocks, t, 0, st>>>(p);
-        else k_add_rmsnorm_grad<1, false, 512, true><<<blocks, t, 0, st>>>(p);
-    } else if (nv == 1) {
-        if (vec) k_add_rmsnorm_grad<1, true, 1024, true><<<blocks, t, 0, st>>>(p);
-        else k_add_rmsnorm_grad<1, false, 1024, true><<<blocks, t, 0, st>>>(p);
-    } else {
-        if (vec) k_add_rmsnorm_grad<4, true, 512, false><<<blocks, t, 0, st>>>(p);
-        else k_add_rmsnorm_grad<4, false, 512, false><<<blocks, t, 0, st>>>(p);
-    }
+    auto launch = [&](auto vectors) {
+        constexpr int NV = decltype(vectors)::value;
+        if (vec) k_add_rmsnorm_grad<NV, true><<<blocks, t, 0, st>>>(p);
+        else k_add_rmsnorm_grad<NV, false><<<blocks, t, 0, st>>>(p);
+    };
+    if (nv == 1) launch(std::integral_constant<int, 1>());
+    else if (nv == 2) launch(std::integral_constant<int, 2>());
+    else launch(std::integral_constant<int, 4>());
     CF_LAUNCH_CHECK("add_rmsnorm_grad");
     if (d_dscale_or_null) {
         k_sum_partials<<<(H + 31) / 32, 1024, 0, st>>>(d_scratch, blocks, H, d_dscale_or_null, accumulate_dscale);

@@ -315,6 +315,13 @@ def test_add_rmsnorm_gradient(cfb, rows, H, with_dh):
         assert torch.equal(into, dx)
 
 
+# every number of vectors a thread holds (by row length and by row count), and blocks that walk several rows
+@pytest.mark.parametrize("rows,H", [(148, 520), (149, 4096), (593, 4096), (15000, 128), (1800, 4104), (1800, 8192), (460, 8200), (300, 4101)])
+def test_add_rmsnorm_many_rows(cfb, rows, H):
+    test_add_rmsnorm_quantise(cfb, rows, H, True)
+    test_add_rmsnorm_gradient(cfb, rows, H, True)
+
+
 def test_add_rmsnorm_gradient_against_differences(cfb):
     """A directional derivative of sum(c * y(h)) in 64 bits against the kernel's gradient."""
     rows, H, eps = 4, 512, 1e-5
