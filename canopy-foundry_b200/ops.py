@@ -581,6 +581,9 @@ def _refuse(what):
     raise CanopyError(_capi.CF_ERR_INVALID_ARG, what)
 
 
+_INT_MAX = 0x7fffffff              # of a C int: ctypes would cut a larger size down without a word
+
+
 def _blocks(n):
     return (n + 127) >> 7
 
@@ -605,6 +608,8 @@ def _mat(t, dtype, rows, cols, what):
     ld, step = t.stride()
     if (step != 1 and cols > 1) or (ld < cols and rows > 1):
         _refuse(f"{what}: columns must be contiguous and rows must not overlap")
+    if rows > _INT_MAX or cols > _INT_MAX or (ld > _INT_MAX and rows > 1):
+        _refuse(f"{what}: sizes and pitches go up to 2^31 - 1")
     return ld if rows > 1 else (cols + 15) & ~15       # the pitch of a single row addresses no memory
 
 
@@ -618,6 +623,8 @@ def _scales(t, rows, cols, what):
 def _dense(t, dtype, shape, what):
     if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
         _refuse(f"{what}: contiguous {dtype} {list(shape)} expected, got {t.dtype} {tuple(t.shape)}")
+    if len(shape) == 2 and max(shape) > _INT_MAX:
+        _refuse(f"{what}: sizes go up to 2^31 - 1")
 
 
 def block128_row_descale(rows, cols, device="cuda"):
@@ -676,6 +683,8 @@ def fp8_quantize_block128x128(w, w8, descale):
     if w.dim() not in (2, 3) or w8.shape != w.shape or descale.dim() != w.dim():
         _refuse("weight, codes and descales: shapes differ")
     n = w.shape[0] if w.dim() == 3 else 1
+    if n > _INT_MAX:
+        _refuse("a stack of more than 2^31 - 1 weights")
     rows, cols = w.shape[-2:]
     if n == 0 or rows == 0 or cols == 0:
         return
@@ -756,6 +765,8 @@ def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_desc
     [E, ceil(N/128), ceil(K/128)]) into the same rows of the bf16 out; the other rows are left as they are."""
     _on(counts, offsets, A8, a_descale, B8, b_descale, out)
     (T, K), (E, N, _) = A8.shape, B8.shape
+    if not 0 < E <= _INT_MAX:
+        _refuse("B8: no experts, or more than 2^31 - 1")
     _dense(counts, _i32, (E,), "counts")
     _dense(offsets, _i32, (E,), "offsets")
     ldb = _mat(B8[0], _u8, N, K, "B8")

@@ -167,6 +167,47 @@ def test_wrappers_refuse_tensors_that_do_not_fit(monkeypatch):
     refused(cfb.gemm_fp8_block128_nt_grouped, ctx, c, c, A, da, E8, dev(2, 2, 2, dtype=f32), dev(300, 256, dtype=f32))
 
 
+def test_wrappers_refuse_sizes_beyond_an_int(monkeypatch):
+    """Sizes and pitches cross to C as ints: 2^32 + 256 would arrive there as 256, a call that looks right."""
+    cfb = package()
+    monkeypatch.setattr(cfb.ops, "_s", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    ctx = type("Ctx", (), {"handle": P})()
+    u8, f32, bf16, far = torch.uint8, torch.float32, torch.bfloat16, (1 << 32) + 256
+
+    def meta(*shape, dtype=bf16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    def big(*shape, dtype=bf16):
+        return dev(of=meta(*shape, dtype=dtype))
+
+    def wide(rows, cols, dtype=bf16):
+        return dev(of=meta(rows, far, dtype=dtype)[:, :cols])
+
+    c8, rd, d = dev(4, 256, dtype=u8), dev(4, 2, dtype=f32), dev(1, 2, dtype=f32)
+    x, out, g = dev(4, 256), dev(4, 4), dev(256)
+    E8, ed = big(far, 1, 128, dtype=u8), big(far, 1, 1, dtype=f32)
+    i = big(far, dtype=torch.int32)
+    for fn, args in ((cfb.fp8_quantize_block128, (wide(4, 256), c8, rd)),
+                     (cfb.fp8_quantize_block128, (x, wide(4, 256, u8), rd)),
+                     (cfb.fp8_quantize_block128, (x, None, None, wide(4, 256, u8), dev(1, 256, dtype=f32))),
+                     (cfb.fp8_quantize_block128, (big(1, far), big(1, far, dtype=u8), big(1, far // 128, dtype=f32))),
+                     (cfb.fp8_quantize_block128, (big(far, 1), big(far, 1, dtype=u8), big(far, 1, dtype=f32))),
+                     (cfb.fp8_quantize_block128x128, (wide(4, 256), c8, d)),
+                     (cfb.fp8_quantize_block128x128, (big(far, 1, 1), big(far, 1, 1, dtype=u8), ed)),
+                     (cfb.add_rmsnorm_quantize_block128, (big(far, 256), None, g, None, None, big(far, 256))),
+                     (cfb.add_rmsnorm_backward, (big(far, 256), big(far, 256), g, big(far, dtype=f32), None, big(far, 256))),
+                     (cfb.gemm_fp8_block128_nt, (ctx, wide(4, 256, u8), rd, c8, d, out)),
+                     (cfb.gemm_fp8_block128_nt, (ctx, c8, rd, c8, d, wide(4, 4))),
+                     (cfb.gemm_fp8_block128_dw, (ctx, c8, dev(1, 256, dtype=f32), wide(4, 4, u8), dev(1, 4, dtype=f32), dev(256, 4, dtype=f32))),
+                     (cfb.gemm_fp8_block128_nt_grouped, (ctx, i, i, dev(4, 128, dtype=u8), dev(4, 1, dtype=f32), E8, ed, dev(4, 1))),
+                     (cfb.gemm_fp8_block128_nt_grouped, (ctx, dev(0, dtype=torch.int32), dev(0, dtype=torch.int32), dev(4, 128, dtype=u8),
+                                                         dev(4, 1, dtype=f32), dev(0, 4, 128, dtype=u8), dev(0, 1, 1, dtype=f32), out))):
+        with pytest.raises(cfb.CanopyError) as e:
+            fn(*args)
+        assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG, fn.__name__
+
+
 def test_wrappers_refuse_tensors_of_another_device(monkeypatch):
     """The call goes to the current device's stream: a tensor on the CPU or on another GPU is refused, by every operator."""
     cfb = package()
