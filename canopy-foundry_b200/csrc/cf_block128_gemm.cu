@@ -12,12 +12,15 @@
 //   warps 1, 3   MMA issuers for even and odd blocks (one elected lane each); warp 1 owns the TMEM allocation
 //   warp 2       scales: global memory -> shared-memory ring
 //   warps 4..11  promotion + epilogue: each owns 32 rows x 128 columns of the CTA's 128 x 256 tile in 128 registers a thread
-// Per block of 128 the MMAs of a CTA need 512 clocks; the promotion needs 64 packed multiply-adds per thread and two warps
-// per scheduler, 128 issue slots, and 128 KB of TMEM reads: it hides behind the MMAs.
+// Per block of 128 the MMAs of a pair take 590 clocks; the promotion's 64 packed multiply-adds a thread, from two warps on every
+// scheduler, keep its fp32 pipe busy for 256 (512 where both operands' scales change inside the tile) and come with 128 KB of
+// TMEM reads per CTA. The two overlap but for the hand-over: 775 clocks a block at 8192^3 (460 to 477 us at the 1.45 to 1.49 GHz
+// that the power cap leaves), 1296 with a scale per column.
 //
-// Narrow form (k_gemm_b128_narrow): few rows of A (tokens), or too few tiles of the wide form to fill the chip. The weights take the MMA's 128-row side and TN tokens its column
-// side, and the contraction is split over a cluster of CTAs whose partial sums meet in distributed shared memory, added in
-// rank order: every weight byte is read once, by enough CTAs to fill the chip, and no atomics are involved.
+// Narrow form (k_gemm_b128_narrow): few rows of A (tokens), or too few tiles of the wide form to fill the chip. The weights take
+// the MMA's 128-row side and TN tokens its column side, and the contraction is split over a cluster of CTAs whose partial sums
+// meet in distributed shared memory, added in rank order: every weight byte is read once, by enough CTAs to fill the chip, and
+// no atomics are involved.
 //
 // Every wait on an mbarrier is bounded: a wait that gives up raises an abort flag, records a code in the context's status
 // word, drains the CTA's own copies and MMAs, frees TMEM and returns.
@@ -335,7 +338,7 @@ k_gemm_b128(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // ------------------------------------------------------------ MMA issuers (leader CTA only)
         // Warp 1 issues the even blocks, warp 3 the odd ones, each into its own TMEM buffer: the two sequences do not depend on
         // each other, and while one warp waits for barriers and commits, the other one's MMAs keep the tensor cores fed. One
-        // issuer for both left them idle for half of the time (1030 clocks a block where its MMAs take 500). The warps stay
+        // issuer for both left them idle for half of the time (1030 clocks a block where its MMAs take 590). The warps stay
         // converged and one elected lane issues: descriptors then live in uniform registers, and a block's four MMAs and the
         // commit take 160 clocks to issue instead of 520 from a lane of its own.
         if (leader) {
