@@ -12,6 +12,8 @@
 // plain form), so every input element is read once whatever the number of outputs. A block owns a tile of 128 columns;
 // a half-warp reads 128 columns of one row (256 contiguous bytes) and holds that row's group, so the row amax is four
 // shuffles; the column amax meets in shared memory across the rows of the tile; the values stay in registers in between.
+// Like the norm and the products these kernels may be scheduled while the kernel before them drains, and wait for it before they
+// touch memory: a feed-forward layer of one token (4096 / 14336, four launches) takes 39.9 us instead of 43.1.
 #include <atomic>
 
 #include "cf_common.cuh"
@@ -50,13 +52,14 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
     f[4] = __uint_as_float(v.z << 16); f[5] = __uint_as_float(v.z & 0xffff0000u);
     f[6] = __uint_as_float(v.w << 16); f[7] = __uint_as_float(v.w & 0xffff0000u);
 }
-// Eight bf16 values of a row as one 16-byte load, or element by element where the row's base or its end forbid that.
+// Eight bf16 values of a row as one 16-byte load, or element by element where the row's base or its end forbid that. Plain loads:
+// read-only ones could be moved ahead of the wait for the grid that writes them.
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int n, bool vec) {
-    if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    if (vec && n >= 8) return *reinterpret_cast<const uint4*>(p);
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        if (e < n) w[e >> 1] |= static_cast<uint32_t>(__ldg(p + e)) << (16 * (e & 1));
+        if (e < n) w[e >> 1] |= static_cast<uint32_t>(p[e]) << (16 * (e & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void store8(uint8_t* p, const uint2& q, int n, bool vec) {
@@ -68,8 +71,8 @@ __device__ __forceinline__ void store8(uint8_t* p, const uint2& q, int n, bool v
 // FMAX / a in two parts: `hi` with 16 significant bits, `lo` the rest to 40 bits. For a bf16 value v (8 bits) v * hi is exact and
 // fma(v, lo, v * hi) the correctly rounded v * FMAX / a, exact where that is representable. That matters: quotients of bf16
 // numbers land exactly between two codes about once in three hundred values (ties go to the even code), and with one rounded
-// factor such a value falls to either side. Price: both groupings of 8192 x 4096 in 33.1 us instead of 28.7 (the kernel is bound
-// by the instructions it issues, not by its 134 MB).
+// factor such a value falls to either side. Price: 15 % of both groupings of 8192 x 4096, 31.7 us (the kernel is bound by the
+// instructions it issues, not by its 134 MB).
 struct Scale2 { float hi, lo; };
 __device__ __forceinline__ Scale2 scale2(float fmax, float a) {
     const float s = __fdiv_rn(fmax, a);
@@ -286,7 +289,8 @@ __device__ __forceinline__ void emit_tile(const QuantParams& p, const Tile& t, i
 
 // Tile of (T / 16) * RPT rows x 128 columns. With column groups the tile has 128 rows. The second launch bound holds the
 // registers down to where enough blocks share an SM to hide the loads: SwiGLU rows, 2039 x 14336: 38.6 us at 64 registers (four
-// blocks of 256 threads), 37.1 at 48, 35.0 at 40 (six); one row a thread instead of two 42.
+// blocks of 256 threads), 37.1 at 48, 35.0 at 40 (six; 33 since the launch overlaps the kernel before it); one row a thread
+// instead of two 42.
 template <int SRC, int T, int RPT, bool ROW, bool COL, bool E5M2>
 __global__ void __launch_bounds__(T, !COL ? (SRC == SRC_SWIGLU ? 1536 : 1024) / T : SRC == SRC_PLAIN ? 3 : 2) k_quant_block128(const QuantParams p) {
     constexpr int RG = T / 16;
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(T, !COL ? (SRC == SRC_SWIGLU ? 1536 : 1024) / 
     const int col = c0 + cg * 8;
     const int n = min(8, p.cols - col);
 
+    pdl_wait();
     uint4 b[SRC == SRC_SWIGLU ? RPT : 1];
     PackedTile<RPT> a;
 #pragma unroll
@@ -331,7 +336,7 @@ __global__ void __launch_bounds__(T, !COL ? (SRC == SRC_SWIGLU ? 1536 : 1024) / 
 // A tile's three inputs wait in shared memory, each thread's own 16-byte pieces (asynchronous copies, no barrier): held in
 // registers they leave room for one block per SM, whose loads and arithmetic then do not overlap. d up is kept in the place of
 // gate and up until d gate has left, so the exponential is taken once. 4096 x 14336, both groupings: 237 us with the inputs in
-// registers, 121 us now.
+// registers, 120 us now.
 constexpr int kGradT = 512, kGradRPT = G / (kGradT / 16);
 constexpr int kGradSmem = 3 * kGradRPT * kGradT * 16;
 template <bool ROW, bool COL, bool E5M2>
@@ -343,6 +348,7 @@ __global__ void __launch_bounds__(kGradT, 2) k_swiglu_grad_block128(const QuantP
     const int c0 = cb * G, r0 = rb * G;
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
     const int col = c0 + cg * 8;                               // cols is a multiple of 128: every vector is whole
+    pdl_wait();
 #pragma unroll
     for (int i = 0; i < kGradRPT; ++i) {
         const int r = r0 + rg + i * RG;
@@ -454,11 +460,12 @@ template <int SRC, int T, int RPT, bool ROW, bool COL>
 int launch_fmt(const QuantParams& p, int e5m2, cudaStream_t st) {
     const long long blocks = tiles(p, (T / 16) * RPT);
     if (!fits(blocks)) return CF_ERR_LIMIT;
+    const dim3 grid(static_cast<unsigned>(blocks));
     if constexpr (SRC == SRC_SWIGLU) {
-        k_quant_block128<SRC, T, RPT, ROW, COL, false><<<static_cast<unsigned>(blocks), T, 0, st>>>(p);       // E4M3 only
+        CF_CUDA(launch_pdl(k_quant_block128<SRC, T, RPT, ROW, COL, false>, grid, dim3(T), 0, st, p));       // E4M3 only
     } else {
-        if (e5m2) k_quant_block128<SRC, T, RPT, ROW, COL, true><<<static_cast<unsigned>(blocks), T, 0, st>>>(p);
-        else k_quant_block128<SRC, T, RPT, ROW, COL, false><<<static_cast<unsigned>(blocks), T, 0, st>>>(p);
+        CF_CUDA(e5m2 ? launch_pdl(k_quant_block128<SRC, T, RPT, ROW, COL, true>, grid, dim3(T), 0, st, p)
+                     : launch_pdl(k_quant_block128<SRC, T, RPT, ROW, COL, false>, grid, dim3(T), 0, st, p));
     }
     CF_LAUNCH_CHECK("quant_block128");
     return CF_OK;
@@ -475,7 +482,7 @@ int launch_grad(const QuantParams& p, cudaStream_t st) {
         CF_CUDA(cudaFuncSetAttribute(k_swiglu_grad_block128<ROW, COL, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradSmem));
         ready[dev & 63].store(1, std::memory_order_release);
     }
-    k_swiglu_grad_block128<ROW, COL, E5M2><<<static_cast<unsigned>(blocks), kGradT, kGradSmem, st>>>(p);
+    CF_CUDA(launch_pdl(k_swiglu_grad_block128<ROW, COL, E5M2>, dim3(static_cast<unsigned>(blocks)), dim3(kGradT), kGradSmem, st, p));
     CF_LAUNCH_CHECK("swiglu_grad_block128");
     return CF_OK;
 }

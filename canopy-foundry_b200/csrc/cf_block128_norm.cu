@@ -15,7 +15,9 @@
 // of one block between its reduction and its second use, 16 neighbouring threads hold one group of 128, and one block
 // barrier per row joins the row sum (two copies of the partial sums alternate, so the next row needs no second barrier).
 // The gain's gradient is summed per block over the block's rows in registers, written as one partial row per block and
-// added up in block order by a second launch: no atomics, so the result does not depend on timing.
+// added up in block order by a second launch: no atomics, so the result does not depend on timing. The launches may be scheduled
+// while the kernel before them drains (they wait for it before they touch memory): the gradient of 8192 x 4096 and its sum take
+// 50 us instead of 53.
 #include <type_traits>
 
 #include "cf_common.cuh"
@@ -98,6 +100,7 @@ template <int NV, bool VEC>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
     __shared__ float s_sum[2][32];
     const int nv = (p.H + 7) / 8;
+    pdl_wait();
     int par = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
         const long long base = row * p.H;
@@ -219,6 +222,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) k_add_rmsnorm_grad(const
     constexpr bool PREFETCH = NV <= 2;
     __shared__ float s_sum[2][32];
     const int nv = (p.H + 7) / 8;
+    pdl_wait();
     float dg[NV][8];
     uint4 gain[NV];
 #pragma unroll
@@ -291,8 +295,9 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) k_add_rmsnorm_grad(const
 }
 
 // out[c] (+)= sum over the partial rows, in row order within each of the 32 warps of a block, then over the warps.
-__global__ void __launch_bounds__(1024) k_sum_partials(const float* __restrict__ partial, int n, int H, float* __restrict__ out, int accumulate) {
+__global__ void __launch_bounds__(1024) k_sum_partials(const float* partial, int n, int H, float* out, int accumulate) {
     __shared__ float s[32][33];
+    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float t = 0.0f;
@@ -336,7 +341,7 @@ int launch_forward(const NormParams& p, cudaStream_t st) {
     // Rounds of 2048 threads, 2.25 of them for 7168 elements: 81 us instead of 75 (9000 rows)
     const long long most = static_cast<long long>(sm_count()) * 3 * (1024 / t);
     const long long grid = p.rows < most ? p.rows : most;
-    k_add_rmsnorm<NV, VEC><<<static_cast<unsigned>(grid), t, 0, st>>>(p);
+    CF_CUDA(launch_pdl(k_add_rmsnorm<NV, VEC>, dim3(static_cast<unsigned>(grid)), dim3(t), 0, st, p));
     CF_LAUNCH_CHECK("add_rmsnorm");
     return CF_OK;
 }
@@ -422,15 +427,15 @@ int cf_add_rmsnorm_backward(const void* d_dy, const void* d_h, const void* d_sca
     const int nv = grad_vec(H), t = threads_for((H + 7) / 8, nv), blocks = grad_blocks(rows, H);
     auto launch = [&](auto vectors) {
         constexpr int NV = decltype(vectors)::value;
-        if (vec) k_add_rmsnorm_grad<NV, true><<<blocks, t, 0, st>>>(p);
-        else k_add_rmsnorm_grad<NV, false><<<blocks, t, 0, st>>>(p);
+        return vec ? launch_pdl(k_add_rmsnorm_grad<NV, true>, dim3(blocks), dim3(t), 0, st, p)
+                   : launch_pdl(k_add_rmsnorm_grad<NV, false>, dim3(blocks), dim3(t), 0, st, p);
     };
-    if (nv == 1) launch(std::integral_constant<int, 1>());
-    else if (nv == 2) launch(std::integral_constant<int, 2>());
-    else launch(std::integral_constant<int, 4>());
+    if (nv == 1) CF_CUDA(launch(std::integral_constant<int, 1>()));
+    else if (nv == 2) CF_CUDA(launch(std::integral_constant<int, 2>()));
+    else CF_CUDA(launch(std::integral_constant<int, 4>()));
     CF_LAUNCH_CHECK("add_rmsnorm_grad");
     if (d_dscale_or_null) {
-        k_sum_partials<<<(H + 31) / 32, 1024, 0, st>>>(d_scratch, blocks, H, d_dscale_or_null, accumulate_dscale);
+        CF_CUDA(launch_pdl(k_sum_partials, dim3((H + 31) / 32), dim3(1024), 0, st, d_scratch, blocks, H, d_dscale_or_null, accumulate_dscale));
         CF_LAUNCH_CHECK("sum_partials");
     }
     return CF_OK;
