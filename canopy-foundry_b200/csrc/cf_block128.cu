@@ -15,6 +15,7 @@
 // Like the norm and the products these kernels may be scheduled while the kernel before them drains, and wait for it before they
 // touch memory: a feed-forward layer of one token (4096 / 14336, four launches) takes 39.9 us instead of 43.1.
 #include <atomic>
+#include <cfloat>
 
 #include "cf_common.cuh"
 #include "cf_internal.cuh"
@@ -116,11 +117,12 @@ __device__ __forceinline__ float rcp(float x) {
     return r;
 }
 // silu(g) * u = g / (1 + exp(-g)) * u. The exponential's argument is cut at 80 (exp stays finite): below, silu is zero to within
-// 1e-33. A NaN in g comes through the other factors.
+// 1e-33. A NaN in g comes through the other factors. The quotient q of an infinite g is held down to the largest finite number
+// in the correction only: the correction is then infinite too, of the same sign, instead of the NaN of inf - inf.
 __device__ __forceinline__ float swiglu(float g, float u) {
     const float d = 1.0f + expf(-fmaxf(g, -80.0f)), r = rcp(d);
     const float q = g * r;
-    return fmaf(fmaf(-d, q, g), r, q) * u;
+    return fmaf(fmaf(-d, fminf(q, FLT_MAX), g), r, q) * u;
 }
 
 // Values of a tile as the emitter wants them: RPT rows x 8 columns per thread. Bf16 sources stay packed (the row is unpacked

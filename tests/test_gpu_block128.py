@@ -216,6 +216,41 @@ def test_swiglu_gradient_quantise(cfb, rows, cols, e5m2):
         assert (decode(codes, e5m2) - want).abs().le(bound).all()
 
 
+def swiglu_codes(cfb, gate, up):
+    """Both groupings of silu(gate) * up: codes and descales of the rows, of the columns."""
+    rows, cols = gate.shape
+    row8, col8 = (torch.empty((rows, cols), dtype=torch.uint8, device="cuda") for _ in range(2))
+    rd, cd = torch.empty((rows, cdiv(cols, G)), device="cuda"), torch.empty((cdiv(rows, G), cols), device="cuda")
+    cfb.swiglu_quantize_block128(gate, up, row8, rd, col8, cd)
+    return row8, rd, col8, cd
+
+
+@pytest.mark.parametrize("rows,cols", [(4, 256), (130, 264), (2500, 2304)])       # every tile size of the kernel
+def test_swiglu_infinite_gate(cfb, rows, cols):
+    """silu(+inf) is +inf: its groups get descale +Inf and contribute NaN, every other group is as it would be without it."""
+    gate, up = normal((rows, cols), 23, 2.0), normal((rows, cols), 24)
+    q0, d0, c0, cd0 = swiglu_codes(cfb, gate, up)
+    only0, od0 = torch.empty_like(q0), torch.empty_like(d0)
+    cfb.swiglu_quantize_block128(gate, up, only0, od0)
+    assert torch.equal(only0, q0) and torch.equal(od0, d0)
+    bad = gate.clone()
+    bad[1, 5] = float("inf")
+    up[1, 5] = -0.25
+    q, d, c, cd = swiglu_codes(cfb, bad, up)
+    only, od = torch.empty_like(q), torch.empty_like(d)
+    cfb.swiglu_quantize_block128(bad, up, only, od)
+    assert torch.equal(only, q) and torch.equal(od, d)
+    assert torch.isinf(d[1, 0]) and torch.isinf(cd[0, 5])
+    assert (decode(q, False)[1, :G] * d[1, 0].double()).isnan().all()
+    assert (decode(c, False)[:min(rows, G), 5] * cd[0, 5].double()).isnan().all()
+    d[1, 0], cd[0, 5] = d0[1, 0], cd0[0, 5]              # the two groups that hold it
+    q[1, :G], c[:G, 5] = q0[1, :G], c0[:G, 5]
+    assert torch.equal(d, d0) and torch.equal(q, q0) and torch.equal(c, c0) and torch.equal(cd, cd0)
+    bad[1, 5], up[1, 5] = float("inf"), 0.0              # infinity times zero: NaN, which the amax ignores
+    q, d, _, _ = swiglu_codes(cfb, bad, up)
+    assert torch.isfinite(d).all() and decode(q, False)[1, 5].isnan() and torch.isfinite(decode(q, False)[1, :5]).all()
+
+
 # ---------------------------------------------------------------- residual + norm
 NORM_SHAPES = [(1, 4096), (3, 1), (5, 100), (2, 129), (65, 512), (33, 1000), (7, 4100), (4, 8193), (3, 16384), (700, 2048)]
 
