@@ -116,11 +116,12 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// silu(g) * u = g / (1 + exp(-g)) * u. The exponential's argument is cut at 80 (exp stays finite): below, silu is zero to within
-// 1e-33. A NaN in g comes through the other factors. The quotient q of an infinite g is held down to the largest finite number
-// in the correction only: the correction is then infinite too, of the same sign, instead of the NaN of inf - inf.
+// silu(g) * u = g / (1 + exp(-g)) * u, with the sum held down to the largest finite number: for g below -87.3 the reciprocal then
+// is zero and so is silu, which is less than 2^-119 there (g multiplies what is left of the sigmoid, so a cut of the exponent
+// alone would leave a value that grows with |g|). The quotient q of an infinite g is held down in the correction only: the correction
+// is then infinite too, of the same sign, instead of the NaN of inf - inf. NaN, and -inf (inf * 0), give NaN.
 __device__ __forceinline__ float swiglu(float g, float u) {
-    const float d = 1.0f + expf(-fmaxf(g, -80.0f)), r = rcp(d);
+    const float d = 1.0f + fminf(expf(-g), FLT_MAX), r = rcp(d);
     const float q = g * r;
     return fmaf(fmaf(-d, fminf(q, FLT_MAX), g), r, q) * u;
 }
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kGradT, 2) k_swiglu_grad_block128(const QuantP
         unpack8(*own[2], d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float ex = expf(-fmaxf(g[e], -80.0f));       // e stays finite: e s is 1, not inf * 0, far below zero
+            const float ex = fminf(expf(-g[e]), FLT_MAX);      // finite: far below zero s is 0 and e s is too, not inf * 0
             const float r0 = rcp(1.0f + ex), sg = fmaf(fmaf(-(1.0f + ex), r0, 1.0f), r0, r0);
             const float ds = d[e] * sg;
             f.v[i][e] = ds * u[e] * fmaf(g[e], ex * sg, 1.0f);

@@ -190,6 +190,61 @@ def test_swiglu_quantise(cfb, rows, cols):
     assert torch.equal(only, row8)
 
 
+FAR = [60.0, -60.0, -80.0, -85.0, -87.0, -88.0, 100.0, -100.0, 1e4, -1e4, 1e30, -1e30, 3e38, -3e38]
+# 1 / (1 + exp(-g)) is taken as zero where it is below the smallest normal number, 2^-126, that is for g below -87.3: there |silu| <
+# 87.4 * 2^-126 < 2^-119, and each gradient's factor is smaller than that
+FLUSHED = 2.0 ** -119
+
+
+def test_swiglu_far_gates(cfb):
+    """Gates far from zero, one in each group of 128 columns, in forward and gradient: right to the bounds of the operator's
+    arithmetic, a vanishing silu times a huge up included."""
+    n = len(FAR)
+    for u in (1.0, -3.0, 1e30):
+        gate = torch.zeros((n, G), dtype=torch.bfloat16, device="cuda")
+        gate[:, 7] = torch.tensor(FAR, device="cuda").to(torch.bfloat16)
+        up, dh = torch.zeros_like(gate), torch.zeros_like(gate)
+        up[:, 7], dh[:, 7] = u, 0.5
+        g, uu, d = (t[:, 7].double() for t in (gate, up, dh))
+        s, rest = torch.sigmoid(g), torch.sigmoid(-g)
+        q, rd, c, _ = swiglu_codes(cfb, gate, up)
+        v = g * s * uu
+        ok = v.abs() < 3e38                              # beyond: not a finite fp32 number
+        a = torch.clamp(v.abs(), min=1e-12)
+        # the descale is the one value's magnitude over 448 (or the floor's), the code +-448 (or, far below the floor, zero)
+        assert (rd[:, 0].double() * 448 - a)[ok].abs().le((SWIGLU_SLACK + 4 * U) * a[ok] + FLUSHED * abs(u)).all(), u
+        got = decode(q, False)[:, 7] * rd[:, 0].double()
+        # the code is off by half a step of the coding at the floor: 2^-10 times 1e-12 / 448
+        assert (got - v)[ok].abs().le((SWIGLU_SLACK + 8 * U) * v[ok].abs() + FLUSHED * abs(u) + HALF[False] * v[ok].abs() * (v[ok].abs() < 1e-12)
+                                      + TINY[False] * 1e-12 / 448).all(), u
+        b8, bd = torch.empty((n, 2 * G), dtype=torch.uint8, device="cuda"), torch.empty((n, 2), device="cuda")
+        cfb.swiglu_backward_quantize_block128(gate, up, dh, b8, bd)
+        got = decode(b8, False)[:, [7, G + 7]] * bd.double()
+        # 1 + g (1 - s): the two terms' magnitudes, where they cancel the error is relative to them
+        want = torch.stack([d * uu * s * (1 + g * rest), d * g * s], 1)
+        size = torch.stack([(d * uu).abs() * s * (1 + (g * rest).abs()), want[:, 1].abs()], 1)
+        room = torch.stack([(d * uu).abs(), d.abs()], 1) * FLUSHED
+        ok = want.abs() < 3e38
+        assert (got - want)[ok].abs().le(((SWIGLU_SLACK + 8 * U) * size + room + HALF[False] * want.abs() * (want.abs() < 1e-12)
+                                          + TINY[False] * 1e-12 / 448)[ok]).all(), u
+
+
+def test_swiglu_gates_without_a_value(cfb):
+    """A NaN gate, and an infinite one where the formula has no value (inf * 0): NaN, in forward and gradient, and nowhere else."""
+    gate, up, dh = normal((3, 256), 25, 2.0), normal((3, 256), 26), normal((3, 256), 27)
+    gate[1, 5], gate[1, 200], gate[2, 9] = float("nan"), float("-inf"), float("inf")
+    q, rd, c, cd = swiglu_codes(cfb, gate, up)
+    v = decode(q, False)
+    assert v[1, 5].isnan() and v[1, 200].isnan() and decode(c, False)[1, [5, 200]].isnan().all() and torch.isfinite(cd[:, 200]).all()
+    assert torch.isfinite(rd[1]).all() and int(v[1].isnan().sum()) == 2 and torch.isfinite(v[0]).all() and torch.isfinite(v[2, 128:]).all()
+    b8, bd = torch.empty((3, 512), dtype=torch.uint8, device="cuda"), torch.empty((3, 4), device="cuda")
+    cfb.swiglu_backward_quantize_block128(gate, up, dh, b8, bd)
+    b = decode(b8, False)
+    assert b[1, [5, 200, 256 + 5, 256 + 200]].isnan().all() and int(b[1].isnan().sum()) == 4 and torch.isfinite(bd[1]).all()
+    assert torch.isfinite(b[0]).all() and b[2, 9].isnan() and int(b[2, :256].isnan().sum()) == 1
+    assert torch.isinf(bd[2, 2]) and (b[2, 256:384] * bd[2, 2].double()).isnan().all()          # d up = dh * inf
+
+
 @pytest.mark.parametrize("e5m2", [False, True])
 @pytest.mark.parametrize("rows,cols", [(1, 128), (129, 384), (300, 1024)])
 def test_swiglu_gradient_quantise(cfb, rows, cols, e5m2):
