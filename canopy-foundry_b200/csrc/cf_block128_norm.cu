@@ -9,7 +9,8 @@
 // not depend on rms: with t = h * scale (exact in fp32, 16 bits) and m = max|t| over the group, y * 448 / a = t * 448 / m. The
 // quotient is taken correctly rounded, exact where it is representable: it lands exactly between two codes about once in a
 // thousand values, and a rounded factor would send such a value to either side.
-// Sums, rms and descales are fp32.
+// Sums, rms and descales are fp32. In a row with an infinity rms is infinite and y is 0, NaN at the infinity itself; a NaN makes
+// its whole row NaN.
 //
 // Both are streams: forward 2+2 B in, 2+1 B out per element (7), backward 2+2+2 in, 2 out (8). A row lives in the registers
 // of one block between its reduction and its second use, 16 neighbouring threads hold one group of 128, and one block
@@ -93,11 +94,51 @@ struct NormParams {
     int vec8;
 };
 
+// 448 / m in two parts, 8 significant bits and the rest: t * hi is exact, fma(t, lo, t * hi) the rounded quotient.
+struct Quotient { float hi, lo; };
+__device__ __forceinline__ Quotient quotient(float m) {
+    const float quot = __fdiv_rn(448.0f, m);
+    const float hi = __uint_as_float(__float_as_uint(quot) & 0xffff0000u);
+    const float rest = fmaf(fmaf(-quot, m, 448.0f), quot * (1.0f / 448.0f), quot - hi);
+    return {hi, isfinite(rest) ? rest : 0.0f};          // a group with an infinity: the quotient is 0
+}
+
+// A row whose rms is not finite, by all threads of its block: y = h / rms is taken before the groups' maxima (with the maxima of
+// h * scale a factor of 1 / rms behind them would be inf * 0 in every group). The row is read again from where h stands, the sum's
+// barrier has made it visible; a call of its own, since the same lines inside the kernel cost every row (16384 x 4096: 84 us
+// instead of 80).
+__device__ __noinline__ void unbounded_row(const NormParams& p, long long row, float rms) {
+    const uint16_t* src = (p.h ? p.h : p.x) + row * p.H;
+    const float inv = __fdiv_rn(1.0f, rms);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
+    for (int group = warp; group * 128 < p.H; group += warps) {      // one warp: 128 values, four a lane
+        float y[4], m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = group * 128 + 32 * e + lane;
+            y[e] = c < p.H ? bf16_bits_to_f32(src[c]) * inv * bf16_bits_to_f32(p.gain[c]) : 0.0f;
+            m = fmaxf(m, fabsf(y[e]));
+        }
+        m = fmaxf(warp_max(m), 1e-12f);
+        const Quotient q = quotient(m);
+        if (p.out8 && lane == 0) p.descale[row * p.d_row + group * p.d_blk] = __fdiv_rn(m, 448.0f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = group * 128 + 32 * e + lane;
+            if (c < p.H) {
+                if (p.normed) p.normed[row * p.H + c] = static_cast<uint16_t>(pack2(y[e], 0.0f));
+                if (p.out8) p.out8[row * p.ld_out8 + c] = cvt_fp8<false>(fmaf(y[e], q.lo, y[e] * q.hi));
+            }
+        }
+    }
+}
+
 // x, res and h may be the same memory (every thread reads its own elements before it writes them, and a row belongs to one
 // block): no __restrict__. A row's loads of x and of the residual are all issued before either is used: 16384 x 4096 takes
 // 78 us (0.92 of the measured copy rate), 89 with the residual's loads behind the use of x's.
 template <int NV, bool VEC>
-__global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
+__global__ void __launch_bounds__(1024) k_add_rmsnorm(const __grid_constant__ NormParams p) {
     __shared__ float s_sum[2][32];
     const int nv = (p.H + 7) / 8;
     pdl_wait();
@@ -137,6 +178,10 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
         }
         const float total = block_sum(acc, s_sum[par]);
         const float rms = sqrtf(__fdiv_rn(total, static_cast<float>(p.H)) + p.eps);
+        if (!isfinite(rms)) {                           // the same in every thread
+            unbounded_row(p, row, rms);
+            continue;
+        }
         if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
         const float inv = __fdiv_rn(1.0f, rms);
         float amax[NV];                                 // of t over the group of 128 that this half-warp holds in vector i
@@ -173,17 +218,13 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const NormParams p) {
             for (int i = 1; i < NV; ++i)
                 if (cg == i) mine = amax[i];
             mine = fmaxf(mine, 1e-12f * rms);           // the floor of max|y|
-            // 448 / m in two parts, 8 significant bits and the rest: t * hi is exact, fma(t, lo, t * hi) the rounded quotient
-            const float quot = __fdiv_rn(448.0f, mine);
-            const float s_hi = __uint_as_float(__float_as_uint(quot) & 0xffff0000u);
-            const float rest = fmaf(fmaf(-quot, mine, 448.0f), quot * (1.0f / 448.0f), quot - s_hi);
-            const float s_lo = isfinite(rest) ? rest : 0.0f;        // a group with an infinity: the quotient is 0
+            const Quotient s = quotient(mine);
             const int my_group = (threadIdx.x + blockDim.x * cg) / 16;
             if (cg < NV && my_group * 16 < nv) p.descale[row * p.d_row + my_group * p.d_blk] = __fdiv_rn(mine * inv, 448.0f);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int vi = threadIdx.x + blockDim.x * i;
-                const float hi = __shfl_sync(0xffffffffu, s_hi, (lane & 16) | i), lo = __shfl_sync(0xffffffffu, s_lo, (lane & 16) | i);
+                const float hi = __shfl_sync(0xffffffffu, s.hi, (lane & 16) | i), lo = __shfl_sync(0xffffffffu, s.lo, (lane & 16) | i);
                 if (vi < nv) {
                     float q[8];
 #pragma unroll

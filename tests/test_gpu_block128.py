@@ -368,6 +368,40 @@ def test_add_rmsnorm_zero_rows_and_row_of_zeros(cfb):
     cfb.add_rmsnorm_quantize_block128(x[:0], None, gain, None, None, None, out8[:0], d[:0])
 
 
+# one vector per thread, two, four, and rows that are not made of whole vectors
+WIDTHS = [(6, 512), (200, 4096), (700, 4096), (5, 16384), (5, 1001)]
+
+
+@pytest.mark.parametrize("rows,H", WIDTHS)
+@pytest.mark.parametrize("residual", [True, False])
+def test_add_rmsnorm_infinities_and_nan(cfb, rows, H, residual):
+    """A row with an infinity: rms is infinite, its y is 0, NaN at the infinity itself; a row with a NaN: NaN throughout. Groups
+    without a finite value other than zero get the descale of the floor. The rows beside them are as they would be alone."""
+    x, r, gain = normal((rows, H), 45), normal((rows, H), 46), normal((H,), 47)
+
+    def run(x):
+        h, normed, rms = (torch.empty_like(x) if residual else None), torch.empty_like(x), torch.empty(rows, device="cuda")
+        out8, d = torch.empty((rows, H), dtype=torch.uint8, device="cuda"), torch.empty((rows, cdiv(H, G)), device="cuda")
+        cfb.add_rmsnorm_quantize_block128(x, r if residual else None, gain, h, rms, normed, out8, d)
+        return (x if h is None else h), normed, rms, decode(out8, False), d
+    h0, n0, rms0, v0, d0 = run(x)
+    bad = x.clone()
+    bad[1, 3], bad[2, H - 1], bad[3, 130] = float("inf"), float("-inf"), float("nan")
+    h, n, rms, v, d = run(bad)
+    assert torch.isinf(h[1, 3]) and torch.isinf(h[2, H - 1]) and h[3, 130].isnan()
+    assert torch.isinf(rms[1:3]).all() and rms[3].isnan()
+    floor = float((torch.tensor(1e-12).double() / 448.0).float())
+    for row, at in ((1, 3), (2, H - 1)):
+        rest = torch.arange(H, device="cuda") != at
+        assert v[row, at].isnan() and v[row][rest].eq(0).all() and d[row].eq(floor).all()
+        assert n[row, at].isnan() and n[row][rest].eq(0).all()
+    assert v[3].isnan().all() and n[3].isnan().all() and d[3].eq(floor).all()
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[1:4] = False
+    for a, b in ((n, n0), (rms, rms0), (v, v0), (d, d0)):
+        assert torch.equal(a[rest], b[rest])
+
+
 def grad64(dy, h, gain, rms, dh):
     dy, xh, g = dy.double(), h.double() / rms.double()[:, None], gain.double()
     u = dy * g
