@@ -9,8 +9,8 @@
 // not depend on rms: with t = h * scale (exact in fp32, 16 bits) and m = max|t| over the group, y * 448 / a = t * 448 / m. The
 // quotient is taken correctly rounded, exact where it is representable: it lands exactly between two codes about once in a
 // thousand values, and a rounded factor would send such a value to either side.
-// Sums, rms and descales are fp32. In a row with an infinity rms is infinite and y is 0, NaN at the infinity itself; a NaN makes
-// its whole row NaN.
+// Sums, rms and descales are fp32; a sum of squares beyond fp32 is taken again over scaled values. In a row with an infinity rms is
+// infinite and y is 0, NaN at the infinity itself; a NaN makes its whole row NaN.
 //
 // Both are streams: forward 2+2 B in, 2+1 B out per element (7), backward 2+2+2 in, 2 out (8). A row lives in the registers
 // of one block between its reduction and its second use, 16 neighbouring threads hold one group of 128, and one block
@@ -103,32 +103,46 @@ __device__ __forceinline__ Quotient quotient(float m) {
     return {hi, isfinite(rest) ? rest : 0.0f};          // a group with an infinity: the quotient is 0
 }
 
-// A row whose rms is not finite, by all threads of its block: y = h / rms is taken before the groups' maxima (with the maxima of
-// h * scale a factor of 1 / rms behind them would be inf * 0 in every group). The row is read again from where h stands, the sum's
-// barrier has made it visible; a call of its own, since the same lines inside the kernel cost every row (16384 x 4096: 84 us
-// instead of 80).
-__device__ __noinline__ void unbounded_row(const NormParams& p, long long row, float rms) {
+// A row whose sum of squares is beyond fp32, by all threads of its block. Values above 1.8e19 alone do that: the sum is taken again
+// over h * 2^-72 (below 2^126 for the longest row of the largest numbers; what loses bits in the scaling is below 2^-110 of the rms),
+// and y = (h 2^-72) / (rms 2^-72) * scale. With an infinity or a NaN in the row that sum is not finite either: y = h / rms * scale
+// is then taken before the groups' maxima (a factor of 1 / rms behind them would be inf * 0 in every group).
+// The row is read again from where h stands, the sum's barrier has made it visible; a call of its own, since lines inside the
+// kernel cost every row (16384 x 4096: 84 us instead of 80).
+__device__ __noinline__ void unbounded_row(const NormParams& p, long long row) {
+    constexpr float kDown = 0x1p-72f, kUp = 0x1p72f;
+    __shared__ float s_again[32];
     const uint16_t* src = (p.h ? p.h : p.x) + row * p.H;
-    const float inv = __fdiv_rn(1.0f, rms);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;
+    float acc = 0.0f;
+    for (int c = threadIdx.x; c < p.H; c += blockDim.x) {
+        const float f = bf16_bits_to_f32(src[c]) * kDown;
+        acc = fmaf(f, f, acc);
+    }
+    float rms = sqrtf(__fdiv_rn(block_sum(acc, s_again), static_cast<float>(p.H)) + p.eps * kDown * kDown);
+    if (threadIdx.x == 0 && p.rms) p.rms[row] = rms * kUp;
+    float inv = __fdiv_rn(1.0f, rms), factor = kDown;        // t = h * factor * scale, y = t * inv
+    if (!isfinite(rms)) {
+        factor = inv;
+        rms = inv = 1.0f;
+    }
     for (int group = warp; group * 128 < p.H; group += warps) {      // one warp: 128 values, four a lane
-        float y[4], m = 0.0f;
+        float t[4], m = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int c = group * 128 + 32 * e + lane;
-            y[e] = c < p.H ? bf16_bits_to_f32(src[c]) * inv * bf16_bits_to_f32(p.gain[c]) : 0.0f;
-            m = fmaxf(m, fabsf(y[e]));
+            t[e] = c < p.H ? bf16_bits_to_f32(src[c]) * factor * bf16_bits_to_f32(p.gain[c]) : 0.0f;
+            m = fmaxf(m, fabsf(t[e]));
         }
-        m = fmaxf(warp_max(m), 1e-12f);
+        m = fmaxf(warp_max(m), 1e-12f * rms);
         const Quotient q = quotient(m);
-        if (p.out8 && lane == 0) p.descale[row * p.d_row + group * p.d_blk] = __fdiv_rn(m, 448.0f);
+        if (p.out8 && lane == 0) p.descale[row * p.d_row + group * p.d_blk] = __fdiv_rn(m * inv, 448.0f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int c = group * 128 + 32 * e + lane;
             if (c < p.H) {
-                if (p.normed) p.normed[row * p.H + c] = static_cast<uint16_t>(pack2(y[e], 0.0f));
-                if (p.out8) p.out8[row * p.ld_out8 + c] = cvt_fp8<false>(fmaf(y[e], q.lo, y[e] * q.hi));
+                if (p.normed) p.normed[row * p.H + c] = static_cast<uint16_t>(pack2(t[e] * inv, 0.0f));
+                if (p.out8) p.out8[row * p.ld_out8 + c] = cvt_fp8<false>(fmaf(t[e], q.lo, t[e] * q.hi));
             }
         }
     }
@@ -179,7 +193,7 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm(const __grid_constant__ No
         const float total = block_sum(acc, s_sum[par]);
         const float rms = sqrtf(__fdiv_rn(total, static_cast<float>(p.H)) + p.eps);
         if (!isfinite(rms)) {                           // the same in every thread
-            unbounded_row(p, row, rms);
+            unbounded_row(p, row);
             continue;
         }
         if (threadIdx.x == 0 && p.rms) p.rms[row] = rms;

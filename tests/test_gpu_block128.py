@@ -402,6 +402,35 @@ def test_add_rmsnorm_infinities_and_nan(cfb, rows, H, residual):
         assert torch.equal(a[rest], b[rest])
 
 
+@pytest.mark.parametrize("rows,H", WIDTHS)
+@pytest.mark.parametrize("residual", [True, False])
+def test_add_rmsnorm_rows_whose_squares_overflow(cfb, rows, H, residual):
+    """Finite values above 1.8e19 have squares beyond fp32: rms, y and codes are right all the same."""
+    eps = 1e-6
+    x, gain = normal((rows, H), 48), normal((H,), 49)
+    r = normal((rows, H), 44)
+    x[0] *= 1e30                                         # all of the row
+    x[1, 3] = 2e19                                       # one value, the others vanish beside it
+    x[2] = 3.3895e38                                     # the largest bf16 number throughout
+    x[3, H - 1], x[3, 0] = -3.3895e38, 1e25
+    x[4, : H // 2] *= 1e18                               # the sum overflows, no square does
+    r[2] = 0.0
+    rms, normed, h = torch.empty(rows, device="cuda"), torch.empty_like(x), torch.empty_like(x) if residual else None
+    out8, d = torch.empty((rows, H), dtype=torch.uint8, device="cuda"), torch.empty((rows, cdiv(H, G)), device="cuda")
+    cfb.add_rmsnorm_quantize_block128(x, r if residual else None, gain, h, rms, normed, out8, d, eps=eps)
+    want_h = (x.float() + r.float()).to(torch.bfloat16) if residual else x
+    assert h is None or torch.equal(h, want_h)
+    y, rms64 = norm64(want_h, gain, eps)
+    # as for ordinary rows: 32 squares per thread, 37 additions behind them, root, quotient and products
+    slack = (32 + 37 + 4) * U
+    assert torch.isfinite(rms).all() and (rms.double() - rms64).abs().le(slack * rms64).all()
+    assert (normed.double() - y).abs().le((2.0 ** -8 + slack) * y.abs() + 1e-38).all()
+    check_groups(out8, d, y, 1, False, slack)
+    only, od = torch.empty_like(out8), torch.empty_like(d)           # in place, the codes alone
+    cfb.add_rmsnorm_quantize_block128(x, r if residual else None, gain, x if residual else None, None, None, only, od, eps=eps)
+    assert torch.equal(only, out8) and torch.equal(od, d)
+
+
 def grad64(dy, h, gain, rms, dh):
     dy, xh, g = dy.double(), h.double() / rms.double()[:, None], gain.double()
     u = dy * g
