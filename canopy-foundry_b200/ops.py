@@ -773,6 +773,8 @@ def gemm_fp8_block128_nt_grouped(ctx, counts, offsets, A8, a_descale, B8, b_desc
     if E > 1:
         if N == 1:
             ldb = B8.stride(0)
+            if ldb > _INT_MAX:
+                _refuse("B8: pitches go up to 2^31 - 1")
         if B8.stride(0) != N * ldb:
             _refuse("B8: the experts must lie behind one another")
     if b_descale.dtype is not _f32 or b_descale.shape != (E, _blocks(N), _blocks(K)) or (b_descale.stride(2) != 1 and b_descale.shape[2] > 1):

@@ -233,3 +233,25 @@ def test_wrappers_refuse_tensors_of_another_device(monkeypatch):
                     with pytest.raises(cfb.CanopyError) as e:
                         fn(*moved)
                     assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG and "device" in str(e.value), (fn.__name__, k)
+
+
+def test_grouped_product_of_single_rows_refuses_a_pitch_beyond_an_int(monkeypatch):
+    """Experts of one row each lie one pitch apart: 2^32 + 256 would reach the library as 256, the rows of other experts."""
+    cfb = package()
+    monkeypatch.setattr(cfb.ops, "_s", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    passed = []
+    fake = type("Lib", (), {"cf_gemm_fp8_block128_nt_grouped": lambda self, *a: passed.append(a) or 0})()
+    monkeypatch.setattr(cfb.ops, "_L", lambda: fake)
+    ctx = type("Ctx", (), {"handle": P})()
+    u8, f32 = torch.uint8, torch.float32
+    i, A, da, db, out = dev(2, dtype=torch.int32), dev(4, 128, dtype=u8), dev(4, 1, dtype=f32), dev(2, 1, 1, dtype=f32), dev(4, 1)
+    for pitch, fits in ((256, True), ((1 << 31) - 16, True), (1 << 31, False), ((1 << 32) + 256, False)):
+        B8 = dev(of=torch.empty((2, 1, pitch), dtype=u8, device="meta")[..., :128])
+        if fits:
+            cfb.gemm_fp8_block128_nt_grouped(ctx, i, i, A, da, B8, db, out)
+            assert passed.pop()[14] == pitch                 # ldb
+        else:
+            with pytest.raises(cfb.CanopyError) as e:
+                cfb.gemm_fp8_block128_nt_grouped(ctx, i, i, A, da, B8, db, out)
+            assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG and not passed
