@@ -1002,7 +1002,7 @@ class FfnSwigluFp8Block128:
             self.n8c, self.a8c = col_codes(H), col_codes(F)
             self.dy8, self.dy8c, self.dgu8, self.dgu8c = codes(H), col_codes(H), codes(2 * F), col_codes(2 * F)
             self.scratch = torch.empty(add_rmsnorm_backward_scratch_floats(R, H), dtype=torch.float32, device=device)
-        self.rows = 0
+        self.rows = None                                 # of the last forward() call that came through
 
     def _rows(self, pair):
         return pair[0][:self.rows], pair[1][:self.rows]
@@ -1013,9 +1013,18 @@ class FfnSwigluFp8Block128:
     def forward(self, x, residual, gain, w_gateup, w_down, y):
         """x, y: bf16 [rows, H]; residual: bf16 [rows, H] or None; w_gateup: Fp8Block128Weight [2F, H] (gate rows first), w_down:
         [H, F]."""
-        rows = self.rows = x.shape[0]
+        rows = x.shape[0]
         if rows > self.max_rows:
             _refuse(f"FfnSwigluFp8Block128: {rows} rows, made for {self.max_rows}")
+        self.rows = rows
+        try:
+            self._forward(x, residual, gain, w_gateup, w_down, y)
+        except BaseException:                            # what the call before it kept has been overwritten in part
+            self.rows = None
+            raise
+
+    def _forward(self, x, residual, gain, w_gateup, w_down, y):
+        rows = self.rows
         n8, dn8 = self._rows(self.n8)
         a8, da8 = self._rows(self.a8)
         gu = self.gu[:rows]
@@ -1037,6 +1046,8 @@ class FfnSwigluFp8Block128:
         dw_gateup [2F, H], dw_down [H, F] (float32 or bf16), dgain (float32 [H]); the last three added to when accumulate."""
         if not self.train:
             _refuse("FfnSwigluFp8Block128: backward() needs train=True")
+        if self.rows is None:
+            _refuse("FfnSwigluFp8Block128: backward() needs a forward() call that came through")
         rows, F, e = self.rows, self.F, self.e5m2
         dy8, ddy8 = self._rows(self.dy8)
         dy8c, ddy8c = self._cols(self.dy8c)

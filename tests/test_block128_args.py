@@ -255,3 +255,43 @@ def test_grouped_product_of_single_rows_refuses_a_pitch_beyond_an_int(monkeypatc
             with pytest.raises(cfb.CanopyError) as e:
                 cfb.gemm_fp8_block128_nt_grouped(ctx, i, i, A, da, B8, db, out)
             assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG and not passed
+
+
+def test_feed_forward_block_after_a_refused_call(monkeypatch):
+    """A call of too many rows changes nothing: backward() still differentiates the call before it. A call that is refused on its
+    way has overwritten what the call before it kept: nothing is left to differentiate."""
+    cfb = package()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    done = []
+    for name in ("add_rmsnorm_quantize_block128", "gemm_fp8_block128_nt", "gemm_fp8_block128_nn", "gemm_fp8_block128_dw", "swiglu_quantize_block128",
+                 "swiglu_backward_quantize_block128", "add_rmsnorm_backward", "fp8_quantize_block128", "fp8_quantize_block128x128"):
+        monkeypatch.setattr(cfb.ops, name, lambda *a, _n=name, **k: done.append((_n, a)))
+    H, F = 256, 128
+    ctx = type("Ctx", (), {"handle": P})()
+    block = cfb.FfnSwigluFp8Block128(ctx, 4, H, F, train=True, device="cpu")
+
+    def bf16(*shape):
+        return torch.empty(shape, dtype=torch.bfloat16)
+
+    wgu, wd = cfb.Fp8Block128Weight(bf16(2 * F, H)), cfb.Fp8Block128Weight(bf16(H, F))
+    gain, dw, dd, dg = bf16(H), torch.empty(2 * F, H), torch.empty(H, F), torch.empty(H)
+
+    def backward(n):
+        done.clear()
+        block.backward(bf16(n, H), None, gain, wgu, wd, bf16(n, H), dw, dd, dg)
+        return [a[1].shape[0] for name, a in done if name == "gemm_fp8_block128_nn"]
+
+    def refused(fn):
+        with pytest.raises(cfb.CanopyError) as e:
+            fn()
+        assert e.value.code == cfb._capi.CF_ERR_INVALID_ARG
+
+    refused(lambda: backward(3))                             # nothing has run
+    block.forward(bf16(3, H), None, gain, wgu, wd, bf16(3, H))
+    assert backward(3) == [3, 3]
+    refused(lambda: block.forward(bf16(5, H), None, gain, wgu, wd, bf16(5, H)))
+    assert backward(3) == [3, 3]
+    monkeypatch.setattr(cfb.ops, "swiglu_quantize_block128", lambda *a: cfb.ops._refuse("on its way"))
+    refused(lambda: block.forward(bf16(2, H), None, gain, wgu, wd, bf16(2, H)))
+    refused(lambda: backward(2))
+    refused(lambda: backward(3))
