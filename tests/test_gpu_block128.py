@@ -154,6 +154,45 @@ def test_quantise_infinities_and_nan(cfb):
     assert torch.equal(row8[3], q[3]) and torch.equal(rd[3], d[3])
 
 
+@pytest.mark.parametrize("e5m2", [False, True])
+@pytest.mark.parametrize("both", [False, True])
+def test_quantise_columns_infinities_and_nan(cfb, e5m2, both):
+    x = normal((200, 136), 6)
+    x[3, 5], x[150, 7], x[60, 130], x[:128, 9] = float("inf"), float("-inf"), float("nan"), float("nan")
+    col8 = torch.empty((200, 136), dtype=torch.uint8, device="cuda")
+    cd = torch.empty((2, 136), device="cuda")
+    row8, rd = (torch.empty_like(col8), torch.empty((200, 2), device="cuda")) if both else (None, None)
+    cfb.fp8_quantize_block128(x, row8, rd, col8, cd, is_e5m2=e5m2)
+    clean = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0)
+    q, d = plain_codes(clean, 0, e5m2)
+    holds = torch.zeros((2, 136), dtype=torch.bool, device="cuda")
+    holds[0, 5] = holds[1, 7] = True
+    assert torch.isinf(cd[holds]).all() and torch.equal(cd[~holds], d[~holds])
+    v = decode(col8, e5m2)
+    assert (v * cd.double().repeat_interleave(G, 0)[:200])[holds.repeat_interleave(G, 0)[:200]].isnan().all()
+    rest = ~(holds.repeat_interleave(G, 0)[:200] | x.isnan())
+    assert torch.equal(col8[rest], q[rest]) and v[x.isnan()].isnan().all()
+
+
+def test_quantise_weight_blocks_infinities_and_nan(cfb):
+    w = normal((260, 300), 12, 0.02)
+    w[5, 200], w[140, 3], w[256:, 256:] = float("-inf"), float("nan"), float("nan")
+    w8, d = torch.empty((260, 300), dtype=torch.uint8, device="cuda"), torch.empty((3, 3), device="cuda")
+    cfb.fp8_quantize_block128x128(w, w8, d)
+    v = decode(w8, False) * d.double().repeat_interleave(G, 0)[:260].repeat_interleave(G, 1)[:, :300]
+    assert torch.isinf(d[0, 1]) and v[:128, 128:256].isnan().all() and int(torch.isinf(d).sum()) == 1
+    assert v[140, 3].isnan() and int(v[128:256, :128].isnan().sum()) == 1
+    assert v[256:, 256:].isnan().all() and d[2, 2] == (torch.tensor(1e-12).double() / 448.0).float()
+    clean = torch.nan_to_num(w, nan=0.0, posinf=0.0, neginf=0.0)
+    c8, cd = torch.empty_like(w8), torch.empty_like(d)
+    cfb.fp8_quantize_block128x128(clean, c8, cd)
+    d[0, 1] = cd[0, 1]
+    assert torch.equal(d, cd)
+    rest = torch.isfinite(w)
+    rest[:128, 128:256] = False
+    assert torch.equal(w8[rest], c8[rest])
+
+
 @pytest.mark.parametrize("shape", [(1, 1), (128, 128), (130, 260), (256, 1000), (5, 129), (3, 130, 140), (2, 128, 256), (4, 1, 16)])
 def test_quantise_weight_blocks_bit_exact(cfb, shape):
     w = normal(shape, 11, 0.02)
@@ -671,6 +710,99 @@ def test_product_dw(cfb, ctx, M, N, T, xe, ye):
     c0 = c.clone()
     cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, c, x_is_e5m2=xe, dy_is_e5m2=ye, accumulate=True)
     assert torch.equal(c, (c0.float() + f).to(torch.bfloat16))
+
+
+# More tiles than the chip holds at once, so that every CTA goes from tile to tile (the stages, barrier phases, TMEM buffers and
+# output boxes carry over): CTA pairs with five tiles each, single CTAs with two; an even and an odd number of blocks of K, and one
+SEVERAL_TILES = [(4999, 4360, 100), (4999, 4360, 400), (4999, 4360, 528), (300, 20000, 300), (300, 20000, 128)]
+
+
+@pytest.mark.parametrize("row_groups", [False, True])
+@pytest.mark.parametrize("M,N,K", SEVERAL_TILES)
+def test_product_nt_several_tiles_each(cfb, ctx, M, N, K, row_groups):
+    per = 1 if row_groups else G
+    A, da = coded(M, K, M + N, 1, G)
+    B, db = coded(N, K, M + K, per, G, std=0.5)
+    a, b = value64(A, da, False, 1, G), value64(B, db, False, per, G).t()
+    out, f = torch.empty((M, N), dtype=torch.bfloat16, device="cuda"), torch.full((M, N), 5.0, device="cuda")
+    cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+    cfb.gemm_fp8_block128_nt(ctx, A, da.t().contiguous().t(), B, db, f)
+    ctx.poll_status()
+    check_product(f, a, b, K)
+    assert torch.equal(out, f.to(torch.bfloat16))
+    del a, b
+    for pad in (0, 1):                                   # whole boxes, and element by element
+        for dtype in (torch.float32, torch.bfloat16):
+            o, raw = pitched(M, N, dtype, pad)
+            cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, o)
+            assert torch.equal(o, f.to(dtype))
+            cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, o, accumulate=True)
+            assert torch.equal(o, (f.to(dtype).float() + f).to(dtype))
+            o.copy_(torch.full((), 0x5a5a if dtype == torch.bfloat16 else 0x5a5a5a5a, device="cuda",
+                               dtype=torch.int16 if dtype == torch.bfloat16 else torch.int32).view(dtype))
+            assert raw.eq(0x5a).all()
+    ctx.poll_status()
+
+
+@pytest.mark.parametrize("counts,tail", [([2431, 2600], 89), ([300, 0, 129, 1, 128, 257, 400, 90, 183], 12)])
+@pytest.mark.parametrize("K", [300, 400])
+def test_product_grouped_several_tiles_each(cfb, ctx, counts, tail, K):
+    """CTA pairs (two large groups) and single CTAs (nine small ones)."""
+    N, E = 4352, len(counts)
+    offsets = np.cumsum([0] + counts[:-1])
+    T = sum(counts) + tail
+    A, da = coded(T, K, 5, 1, G)
+    stack = [coded(N, K, 300 + 2 * e, G, G) for e in range(E)]
+    B = torch.stack([torch.nn.functional.pad(s[0], (0, -K % 16)) for s in stack])[..., :K]
+    db = torch.stack([s[1] for s in stack])
+    ct, ot = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (counts, offsets))
+    a = value64(A, da, False, 1, G)
+    for pad in (0, 8, 3):
+        out, raw = pitched(T, N, torch.bfloat16, pad)
+        cfb.gemm_fp8_block128_nt_grouped(ctx, ct, ot, A, da, B, db, out)
+        ctx.poll_status()
+        for e, (o, n) in enumerate(zip(offsets, counts)):
+            if n:
+                check_product(out[o:o + n], a[o:o + n], value64(B[e], db[e], False, G, G).t(), K)
+                out[o:o + n] = torch.full((), 0x5a5a, dtype=torch.int16, device="cuda").view(torch.bfloat16)
+        assert raw.eq(0x5a).all()
+
+
+def test_product_gradients_several_tiles_each(cfb, ctx):
+    """Data and weight gradient with two or three tiles to a CTA pair and an odd number of blocks."""
+    M, N, K = 2300, 4112, 300
+    A, da = coded(M, K, 16, 1, G, e5m2=True)
+    B, db = coded(K, N, 17, G, G)
+    for pad in (0, 1):
+        f, _ = pitched(M, N, torch.float32, pad)
+        cfb.gemm_fp8_block128_nn(ctx, A, da, B, db, f, a_is_e5m2=True)
+        check_product(f, value64(A, da, True, 1, G), value64(B, db, False, G, G), K)
+        out, _ = pitched(M, N, torch.bfloat16, pad)
+        cfb.gemm_fp8_block128_nn(ctx, A, da, B, db, out, a_is_e5m2=True)
+        assert torch.equal(out, f.to(torch.bfloat16))
+    M, T = 2304, 620
+    X, dx = coded(T, M, 18, G, 1)
+    Y, dy = coded(T, N, 19, G, 1, e5m2=True)
+    for pad in (0, 1):
+        f, _ = pitched(M, N, torch.float32, pad)
+        cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, f, dy_is_e5m2=True)
+        check_product(f, value64(X, dx, False, G, 1).t(), value64(Y, dy, True, G, 1), T)
+        g = f.clone()
+        cfb.gemm_fp8_block128_dw(ctx, X, dx, Y, dy, g, dy_is_e5m2=True, accumulate=True)
+        assert torch.equal(g, f + f)
+    ctx.poll_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(8500, 17000, 4096), (4200, 16000, 4224)])
+def test_product_nt_weights_larger_than_the_cache(cfb, ctx, M, N, K):
+    """Products that walk their tiles in bands of 32 and of 16 row blocks, one band and a piece: rows of every block against 64 bits."""
+    A, da = coded(M, K, M + N, 1, G)
+    B, db = coded(N, K, M + K, G, G, std=0.5)
+    out = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    cfb.gemm_fp8_block128_nt(ctx, A, da, B, db, out)
+    ctx.poll_status()
+    rows = torch.cat([torch.arange(3, M, 128, device="cuda"), torch.tensor([0, M - 1], device="cuda")])     # both CTAs of every pair
+    check_product(out[rows], value64(A[rows], da[rows], False, 1, G), value64(B, db, False, G, G).t(), K)
 
 
 def test_empty_sizes_do_nothing(cfb, ctx):
