@@ -12,8 +12,8 @@
 // plain form), so every input element is read once whatever the number of outputs. A block owns a tile of 128 columns;
 // a half-warp reads 128 columns of one row (256 contiguous bytes) and holds that row's group, so the row amax is four
 // shuffles; the column amax meets in shared memory across the rows of the tile; the values stay in registers in between.
-// Like the norm and the products these kernels may be scheduled while the kernel before them drains, and wait for it before they
-// touch memory: a feed-forward layer of one token (4096 / 14336, four launches) takes 39.9 us instead of 43.1.
+// Like the norm and the products these kernels, but for the one for weights, may be scheduled while the kernel before them drains, and
+// wait for it before they touch memory: a feed-forward layer of one token (4096 / 14336, four launches) takes 39.9 us instead of 43.1.
 #include <atomic>
 #include <cfloat>
 
@@ -72,8 +72,8 @@ __device__ __forceinline__ void store8(uint8_t* p, const uint2& q, int n, bool v
 // FMAX / a in two parts: `hi` with 16 significant bits, `lo` the rest to 40 bits. For a bf16 value v (8 bits) v * hi is exact and
 // fma(v, lo, v * hi) the correctly rounded v * FMAX / a, exact where that is representable. That matters: quotients of bf16
 // numbers land exactly between two codes about once in three hundred values (ties go to the even code), and with one rounded
-// factor such a value falls to either side. Price: 15 % of both groupings of 8192 x 4096, 31.7 us (the kernel is bound by the
-// instructions it issues, not by its 134 MB).
+// factor such a value falls to either side. Price: 15 % of both groupings of 8192 x 4096, 32.5 us (67 to 70 % of the issue
+// slots; its 136 MB take 20.8).
 struct Scale2 { float hi, lo; };
 __device__ __forceinline__ Scale2 scale2(float fmax, float a) {
     const float s = __fdiv_rn(fmax, a);
@@ -109,8 +109,10 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// Reciprocal good to one unit in the last place, one instruction. With one correction step it is as good as the IEEE division,
-// whose ten instructions put the SwiGLU forms at the issue limit.
+// Reciprocal good to one unit in the last place, one instruction. A Newton step on it, or on a quotient's remainder taken with a
+// fused multiply-add (P. W. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, IBM J. Res. Dev.
+// 34, 1990), squares the error: what is left before the last rounding is below 2^-44, so the result is the rounded quotient but for
+// values that close to the middle of two numbers.
 __device__ __forceinline__ float rcp(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -292,8 +294,8 @@ __device__ __forceinline__ void emit_tile(const QuantParams& p, const Tile& t, i
 
 // Tile of (T / 16) * RPT rows x 128 columns. With column groups the tile has 128 rows. The second launch bound holds the
 // registers down to where enough blocks share an SM to hide the loads: SwiGLU rows, 2039 x 14336: 38.6 us at 64 registers (four
-// blocks of 256 threads), 37.1 at 48, 35.0 at 40 (six; 33 since the launch overlaps the kernel before it); one row a thread
-// instead of two 42.
+// blocks of 256 threads), 37.1 at 48, 35.0 at 40 (six); one row a thread instead of two 42. As it is 35.4 us, since gates of any
+// size are right.
 template <int SRC, int T, int RPT, bool ROW, bool COL, bool E5M2>
 __global__ void __launch_bounds__(T, !COL ? (SRC == SRC_SWIGLU ? 1536 : 1024) / T : SRC == SRC_PLAIN ? 3 : 2) k_quant_block128(const QuantParams p) {
     constexpr int RG = T / 16;
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(T, !COL ? (SRC == SRC_SWIGLU ? 1536 : 1024) / 
 // A tile's three inputs wait in shared memory, each thread's own 16-byte pieces (asynchronous copies, no barrier): held in
 // registers they leave room for one block per SM, whose loads and arithmetic then do not overlap. d up is kept in the place of
 // gate and up until d gate has left, so the exponential is taken once. 4096 x 14336, both groupings: 237 us with the inputs in
-// registers, 120 us now.
+// registers, 120 to 132 us now (by the box).
 constexpr int kGradT = 512, kGradRPT = G / (kGradT / 16);
 constexpr int kGradSmem = 3 * kGradRPT * kGradT * 16;
 template <bool ROW, bool COL, bool E5M2>

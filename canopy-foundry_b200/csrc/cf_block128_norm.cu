@@ -18,7 +18,7 @@
 // The gain's gradient is summed per block over the block's rows in registers, written as one partial row per block and
 // added up in block order by a second launch: no atomics, so the result does not depend on timing. The launches may be scheduled
 // while the kernel before them drains (they wait for it before they touch memory): the gradient of 8192 x 4096 and its sum take
-// 50 us instead of 53.
+// 50 us instead of 53 (52 on another box).
 #include <type_traits>
 
 #include "cf_common.cuh"
@@ -150,7 +150,7 @@ __device__ __noinline__ void unbounded_row(const NormParams& p, long long row) {
 
 // x, res and h may be the same memory (every thread reads its own elements before it writes them, and a row belongs to one
 // block): no __restrict__. A row's loads of x and of the residual are all issued before either is used: 16384 x 4096 takes
-// 78 us (0.92 of the measured copy rate), 89 with the residual's loads behind the use of x's.
+// 78 to 80 us (0.90 to 0.92 of the measured copy rate), 89 with the residual's loads behind the use of x's.
 template <int NV, bool VEC>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm(const __grid_constant__ NormParams p) {
     __shared__ float s_sum[2][32];

@@ -976,8 +976,9 @@ class FfnSwigluFp8Block128:
     """Pre-norm SwiGLU feed-forward block on a residual stream with block-scaled FP8 products:
         h = x + residual;  n = rmsnorm(h) * gain;  g, u = n . w_gateup^T;  y = (silu(g) * u) . w_down^T
     `h` (the stream behind the addition) stays in self.h for the next layer. Up to max_rows rows a call: one token of a serving
-    step as well as a training batch. train=True keeps what backward() needs; F must then be a multiple of 128. Gradients are
-    coded as E5M2 (grad_e5m2) or E4M3. The buffers belong to the object: one call at a time."""
+    step as well as a training batch. train=True keeps what backward() needs; F must then be a multiple of 128. The column codes of n
+    for the weight gradient are then taken from n's bf16 copy (one rounding more than the row codes have, and 2 + 2 bytes per element).
+    Gradients are coded as E5M2 (grad_e5m2) or E4M3. The buffers belong to the object: one call at a time."""
 
     def __init__(self, ctx, max_rows, H, F, train=False, grad_e5m2=True, eps=1e-6, device="cuda"):
         if train and F % BLOCK:

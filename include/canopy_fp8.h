@@ -459,11 +459,12 @@ int cf_swiglu_quantize_e4m3_record(const void* d_gate, const void* d_up, int ld_
  * addressed by strides in elements, so they may lie [rows, groups], [groups, rows] (what coalesces best in the GEMM) or
  * inside larger buffers: row descale of (r, b) at d[r * ld_row + b * ld_block], column descale of (b, c) at
  * d[b * ld_block + c * ld_col]. NaN is ignored by the amax and coded as NaN; a group that holds an infinity gets descale +Inf
- * and contributes NaN. Any number of rows and columns and any pitch; 16-byte aligned inputs with pitches that are multiples
- * of 8 elements, and 8-byte aligned codes with pitches that are multiples of 8, take vector accesses. The GEMMs need
- * 16-byte aligned codes with pitches that are multiples of 16 (the columns behind a row's end are not read). The current
- * device must be the one the memory (and the context) belongs to. Calls keep nothing from one to the next: any number of them
- * may overlap on several streams and share a context. */
+ * and contributes NaN (v is the value that is coded: silu(gate) * up and its gradient are NaN where their formula is inf * 0, in
+ * fp32; silu and its derivative count as zero below -87.3). Any number of rows and columns and any pitch; 16-byte aligned inputs
+ * with pitches that are multiples of 8 elements, and 8-byte aligned codes with pitches that are multiples of 8, take vector
+ * accesses. The GEMMs need 16-byte aligned codes with pitches that are multiples of 16 (the columns behind a row's end are not
+ * read). The current device must be the one the memory (and the context) belongs to. Calls keep nothing from one to the next: any
+ * number of them may overlap on several streams and share a context. */
 
 /* bf16 [rows, cols] (pitch ld_x) -> codes with row groups and / or codes with column groups, from one read. A pair of
  * codes and descales is left out by passing NULL for both. */
@@ -496,7 +497,9 @@ int cf_fp8_quantize_block128x128(const void* d_w, int ld_w, long long w_stride, 
  *   h = bf16(x + residual); rms = sqrt(mean(h^2) + eps); y = (h / rms) * scale; codes and descales of y
  * x, residual, h, normed: bf16 [rows, H] contiguous, scale bf16 [H], rms float[rows]. Without a residual h = x and d_h may be
  * NULL. h may be the same memory as x or residual. y goes to the codes from fp32; d_normed_or_null receives bf16(y) (the
- * codes may then be left out). eps > 0. At most 16384 elements a row. */
+ * codes may then be left out). eps > 0. At most 16384 elements a row. Any finite h: a sum of squares beyond fp32 is taken over
+ * scaled values. With an infinity in a row rms is +Inf and y is 0, NaN at the infinity itself; with a NaN the row's rms and y
+ * are NaN. */
 int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_null, const void* d_scale, void* d_h_or_null,
                                      void* d_normed_or_null, float* d_rms_or_null, void* d_out8_or_null, int ld_out8, float* d_descale,
                                      long long descale_ld_row, long long descale_ld_block, int rows, int H, float eps, void* stream);
@@ -526,8 +529,8 @@ int cf_gemm_fp8_block128_nt(cf_ctx* ctx, int M, int N, int K, const void* d_A, i
  * the stacked weights [num_experts * N, K] (row pitch ldb), whose descales lie [ceil(N/128), ceil(K/128)] with row pitch
  * b_descale_ld_row and unit block stride, b_descale_stride apart per expert. All compact buffers have max_total_rows rows;
  * rows outside of them are never touched (a group is cut to them, one that starts outside is skipped), rows of no group are
- * left as they are; groups must not overlap. At most 65536 experts. bf16 output, forward only: the weight gradient of a ragged
- * group would need its tokens padded to blocks of 128. */
+ * left as they are; groups must not overlap. K at least 1. At most 65536 experts. bf16 output. Forward only: neither gradient has
+ * a ragged form (the weight gradient's would need every group's tokens padded to blocks of 128). */
 int cf_gemm_fp8_block128_nt_grouped(cf_ctx* ctx, int num_experts, int max_total_rows, int N, int K, const int* d_counts,
                                     const int* d_offsets, const void* d_A, int lda, int a_is_e5m2, const float* d_a_descale,
                                     long long a_descale_ld_row, long long a_descale_ld_block, const void* d_B, int ldb,
