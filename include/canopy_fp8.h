@@ -497,9 +497,9 @@ int cf_fp8_quantize_block128x128(const void* d_w, int ld_w, long long w_stride, 
  *   h = bf16(x + residual); rms = sqrt(mean(h^2) + eps); y = (h / rms) * scale; codes and descales of y
  * x, residual, h, normed: bf16 [rows, H] contiguous, scale bf16 [H], rms float[rows]. Without a residual h = x and d_h may be
  * NULL. h may be the same memory as x or residual. y goes to the codes from fp32; d_normed_or_null receives bf16(y) (the
- * codes may then be left out). eps > 0. At most 16384 elements a row. Any finite h: a sum of squares beyond fp32 is taken over
- * scaled values. With an infinity in a row rms is +Inf and y is 0, NaN at the infinity itself; with a NaN the row's rms and y
- * are NaN. */
+ * codes may then be left out). eps > 0. At most 16384 elements a row. h * scale has to be finite in fp32; a sum of squares beyond
+ * fp32 is taken over scaled values. With an infinity in a row rms is +Inf and y is 0, NaN at the infinity itself; with a NaN the
+ * row's rms and y are NaN. */
 int cf_add_rmsnorm_quantize_block128(const void* d_x, const void* d_residual_or_null, const void* d_scale, void* d_h_or_null,
                                      void* d_normed_or_null, float* d_rms_or_null, void* d_out8_or_null, int ld_out8, float* d_descale,
                                      long long descale_ld_row, long long descale_ld_block, int rows, int H, float eps, void* stream);
